@@ -254,6 +254,53 @@ int onpu_attn_step_dev(const float * q, int Hq, int D, const void * K, const voi
                        int64_t hs, int64_t rs, const float * mask, const float * sinks, float scale, float * out,
                        void * ws, int64_t ws_bytes, void * stream);
 
+/* ---- 8-bit key-value cache on the GPU (no counterpart in the reference, whose cache is the
+ * framework's bf16 / fp32 tensors, model.py:481-528). One layer's keys and values in pages of 64
+ * tokens, int8 codes with one fp32 scale per (page, kv head, K | V); value = code * scale. D a multiple
+ * of 16 up to 256.
+ *   codes  int8 [pages][Hkv][2][64 D], 16-byte aligned. K of a head (index 0): [4][D / 16][16 tokens]
+ *          [16 d], token 16 a + b at [a][.][b][.]; V (index 1): [D / 16][4][16 d][4][4], token
+ *          16 a + 4 b + c at [.][b][.][a][c].
+ *   scales fp32 [pages][Hkv][2]
+ *   table  int32 [nseq][P], rows tld apart: the page of a sequence's positions [64 p, 64 p + 64). An
+ *          entry outside [0, pages), or a position past P pages, is no page: what is written there is
+ *          dropped, what is read or attended from there is NaN.
+ *   off    int32 [nseq + 1]: sequence i has the call's rows [off[i], off[i + 1]) of T; NULL: max_n rows
+ *          each (T = nseq max_n). max_n: at least the longest; rows of a sequence past max_n, and rows
+ *          behind off[nseq], are not touched.
+ * table, pos, lens and off are read by the kernels, not by the host: the calls can be captured and
+ * replayed with other values in them. On `stream`; nothing is allocated. 0 ok, -1 error
+ * (onpu_last_error), nothing launched then. */
+/* quantise k, v [T][Hkv][D] (fp32, or bf16 with kv_bf16; row and head strides in elements, on 16
+ * bytes) into positions [pos[i], pos[i] + n_i) of each sequence. Per touched page, head and K | V:
+ * s = max(max |x| of the new values, 2^-96) / 127; a page that holds earlier tokens of the sequence
+ * (positions below pos[i]) keeps its scale where that is larger, else its codes c become
+ * rne(c * (old s / s), in 64 bits). New codes are rne(x / s) of the exact quotient, ties to even;
+ * slots behind the last token of a page begun here hold 0. A value that is not finite makes the
+ * scale NaN, and with it all that is read of that page, head and K | V, until the page is begun anew.
+ * A page must not be written for two sequences (or twice) in one call. */
+int onpu_kv8_write_dev(void * codes, float * scales, int64_t pages, int Hkv, int D, const void * k, const void * v,
+                       int kv_bf16, int64_t krs, int64_t khs, int64_t vrs, int64_t vhs, const int32_t * table, int64_t tld,
+                       int P, const int32_t * pos, const int32_t * off, int nseq, int64_t T, int max_n, void * stream);
+/* the values of positions [pos[i], pos[i] + n_i): k, v [T][Hkv][D] contiguous, fp32 or bf16, 16-byte
+ * aligned */
+int onpu_kv8_read_dev(const void * codes, const float * scales, int64_t pages, int Hkv, int D, const int32_t * table,
+                      int64_t tld, int P, const int32_t * pos, const int32_t * off, int nseq, int64_t T, int max_n, void * k,
+                      void * v, int kv_bf16, void * stream);
+/* attention of q [T][Hq][D] (fp32, or bf16 with q_bf16; strides as k's) over the cache, out [T][Hq][D]
+ * contiguous in q's type. lens[i]: tokens of sequence i in the cache, its n_i query tokens the last of
+ * them: query j is at position p = lens[i] - n_i + j and sees the positions t <= p, with window > 0
+ * those with t > p - window alone. Score scale * q . K_t + mask[i][t] (mask fp32 [nseq][mld], rows of
+ * max_len or more values, or NULL); sinks fp32 [Hq] or NULL: a logit per head without a value. A query
+ * for which no position has a weight gives zeros. max_len: at least the longest of lens; a sequence
+ * with more gives NaN. ws: onpu_kv8_attn_ws_bytes bytes (0: none needed), 16-byte aligned; calls in
+ * flight together need their own. */
+int64_t onpu_kv8_attn_ws_bytes(int Hq, int D, int Hkv, int nseq, int64_t T, int max_n, int max_len, int window);
+int onpu_kv8_attn_dev(const void * q, int q_bf16, int Hq, int64_t qrs, int64_t qhs, const void * codes, const float * scales,
+                      int64_t pages, int Hkv, int D, const int32_t * table, int64_t tld, int P, const int32_t * lens,
+                      const int32_t * off, int nseq, int64_t T, int max_n, int max_len, const float * mask, int64_t mld,
+                      const float * sinks, int window, float scale, void * out, void * ws, int64_t ws_bytes, void * stream);
+
 /* ---- chained decode GEMVs (no counterpart in the reference's ABI; the reference's fused decode
  * engine likewise runs a token's products in one NPU dispatch). A chain is n dense GEMVs
  * y_i [M][N_i] = x_i [M][K_i] . W_i^T fixed at creation (handles, x and y device pointers; one

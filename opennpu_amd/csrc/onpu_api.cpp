@@ -1902,6 +1902,104 @@ int onpu_attn_step_dev(const float * q, int Hq, int D, const void * K, const voi
     return 0;
 }
 
+// ---- the 8-bit key-value cache. What the three calls check of their cache, table and rows alike
+static bool kv8_fill(const char * name, const void * codes, const float * scales, int64_t pages, int Hkv, int D,
+                     const int32_t * table, int64_t tld, int P, const int32_t * pos, const int32_t * off, int nseq, int64_t T,
+                     int max_n, Kv8Cache & c, Kv8Table & t) {
+    const char * why = nullptr;
+    if (!codes || !scales || !table || !pos) why = "a null pointer";
+    else if (D <= 0 || D > KV8_MAX_D || D % 16 != 0) why = "D a multiple of 16 up to 256";
+    else if (Hkv <= 0 || pages <= 0 || pages > INT32_MAX) why = "Hkv and pages positive, pages below 2^31";
+    else if (((uintptr_t) codes % 16) || ((uintptr_t) scales % 8)) why = "codes 16-byte aligned, scales 8-byte aligned";
+    else if (P <= 0 || nseq < 0 || T < 0 || max_n < 0 || (nseq > 1 && tld < P)) why = "a table of P >= 1 columns, rows P or more apart";
+    else if (T > 0 && (nseq < 1 || max_n < 1)) why = "rows without a sequence, or max_n below 1";
+    else if (!off && T != (int64_t) nseq * max_n) why = "T = nseq max_n rows where off is null";
+    if (why) {
+        g_err = std::string(name) + ": needs " + why;
+        return false;
+    }
+    c = Kv8Cache{(int8_t *) codes, (float *) scales, (int) pages, Hkv, D};
+    t = Kv8Table{table, pos, off, tld, T, P, nseq, max_n};
+    return true;
+}
+
+// whether rows and heads of `bytes`-wide values start on 16 bytes
+static bool kv8_rows_ok(const void * p, int64_t rs, int64_t hs, int bytes) {
+    return p && (uintptr_t) p % 16 == 0 && rs * bytes % 16 == 0 && hs * bytes % 16 == 0;
+}
+
+static int kv8_done(const char * name, hipError_t e) {
+    if (e == hipSuccess) return 0;
+    set_err(name, e);
+    return -1;
+}
+
+int onpu_kv8_write_dev(void * codes, float * scales, int64_t pages, int Hkv, int D, const void * k, const void * v,
+                       int kv_bf16, int64_t krs, int64_t khs, int64_t vrs, int64_t vhs, const int32_t * table, int64_t tld,
+                       int P, const int32_t * pos, const int32_t * off, int nseq, int64_t T, int max_n, void * stream) {
+    Kv8Cache c;
+    Kv8Table t;
+    if (!kv8_fill("onpu_kv8_write_dev", codes, scales, pages, Hkv, D, table, tld, P, pos, off, nseq, T, max_n, c, t)) return -1;
+    if (T == 0) return 0;
+    const int b = kv_bf16 ? 2 : 4;
+    if (T == 1) krs = vrs = 0;                                   // (the stride of one row or head means nothing)
+    if (Hkv == 1) khs = vhs = 0;
+    if ((kv_bf16 != 0 && kv_bf16 != 1) || !kv8_rows_ok(k, krs, khs, b) || !kv8_rows_ok(v, vrs, vhs, b)) {
+        set_err("onpu_kv8_write_dev: needs k and v fp32 or bf16, their rows and heads on 16 bytes");
+        return -1;
+    }
+    return kv8_done("onpu_kv8_write_dev (pages of a sequence times Hkv, or nseq, past a grid)",
+                    launch_kv8_write(c, t, k, v, !kv_bf16, krs, khs, vrs, vhs, (hipStream_t) stream));
+}
+
+int onpu_kv8_read_dev(const void * codes, const float * scales, int64_t pages, int Hkv, int D, const int32_t * table,
+                      int64_t tld, int P, const int32_t * pos, const int32_t * off, int nseq, int64_t T, int max_n, void * k,
+                      void * v, int kv_bf16, void * stream) {
+    Kv8Cache c;
+    Kv8Table t;
+    if (!kv8_fill("onpu_kv8_read_dev", codes, scales, pages, Hkv, D, table, tld, P, pos, off, nseq, T, max_n, c, t)) return -1;
+    if (T == 0) return 0;
+    if ((kv_bf16 != 0 && kv_bf16 != 1) || !kv8_rows_ok(k, 0, 0, 4) || !kv8_rows_ok(v, 0, 0, 4)) {
+        set_err("onpu_kv8_read_dev: needs k and v fp32 or bf16, 16-byte aligned");
+        return -1;
+    }
+    return kv8_done("onpu_kv8_read_dev (pages of a sequence times Hkv, or nseq, past a grid)",
+                    launch_kv8_read(c, t, k, v, !kv_bf16, (hipStream_t) stream));
+}
+
+int64_t onpu_kv8_attn_ws_bytes(int Hq, int D, int Hkv, int nseq, int64_t T, int max_n, int max_len, int window) {
+    if (Hq <= 0 || D <= 0 || Hkv <= 0 || Hq % Hkv || nseq <= 0 || T <= 0 || max_n <= 0 || max_len <= 0) return 0;
+    return kv8_attn_ws_bytes(Hq, D, Hkv, nseq, T, max_n, max_len, window);
+}
+
+int onpu_kv8_attn_dev(const void * q, int q_bf16, int Hq, int64_t qrs, int64_t qhs, const void * codes, const float * scales,
+                      int64_t pages, int Hkv, int D, const int32_t * table, int64_t tld, int P, const int32_t * lens,
+                      const int32_t * off, int nseq, int64_t T, int max_n, int max_len, const float * mask, int64_t mld,
+                      const float * sinks, int window, float scale, void * out, void * ws, int64_t ws_bytes, void * stream) {
+    Kv8Cache c;
+    Kv8Table t;
+    if (!kv8_fill("onpu_kv8_attn_dev", codes, scales, pages, Hkv, D, table, tld, P, lens, off, nseq, T, max_n, c, t)) return -1;
+    if (T == 0) return 0;
+    if (Hq <= 0 || Hq % Hkv || max_len < 1 || window < 0 || (mask && mld < max_len)) {
+        set_err("onpu_kv8_attn_dev: needs Hq a multiple of Hkv, max_len >= 1, window >= 0, mask rows of max_len or more");
+        return -1;
+    }
+    if (T == 1) qrs = 0;
+    if (Hq == 1) qhs = 0;
+    if ((q_bf16 != 0 && q_bf16 != 1) || !kv8_rows_ok(q, qrs, qhs, q_bf16 ? 2 : 4) || !kv8_rows_ok(out, 0, 0, 4)) {
+        set_err("onpu_kv8_attn_dev: needs q and out fp32 or bf16, rows and heads on 16 bytes");
+        return -1;
+    }
+    const int64_t need = kv8_attn_ws_bytes(Hq, D, Hkv, nseq, T, max_n, max_len, window);
+    if (need > 0 && (!ws || ws_bytes < need || (uintptr_t) ws % 16)) {
+        set_err("onpu_kv8_attn_dev: needs a 16-byte aligned workspace of onpu_kv8_attn_ws_bytes");
+        return -1;
+    }
+    return kv8_done("onpu_kv8_attn_dev (rows times heads, or nseq, past a grid)",
+                    launch_kv8_attn(c, t, q, !q_bf16, Hq, qrs, qhs, max_len, mask, mld, sinks, window, scale, out, ws,
+                                    (hipStream_t) stream));
+}
+
 int onpu_transcode_q4k_dev(void * h, int64_t e0, int64_t n, const void * blocks, int64_t ld, void * stream) {
     auto * m = (Mat4 *) h;
     if (!m || !blocks || m->fmt != ONPU_Q4NX || m->K % 256 != 0 || e0 < 0 || n < 0 || e0 + n > m->E ||

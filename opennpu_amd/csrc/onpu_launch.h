@@ -4,6 +4,7 @@
 #include <stdint.h>
 
 #include "onpu_common.h"
+#include "onpu_kv8.h"
 
 // k_qgemv: y = x . deq(W)^T for M <= 64 rows of x, per slot (expert) and epilogue
 struct QArgs {
@@ -273,6 +274,14 @@ int64_t attn_ws_bytes(int Hq, int D, int Hkv, int64_t S);
 hipError_t launch_attn_step(const float * q, int Hq, int D, const void * K, const void * V, int kv_bf16, int Hkv,
                             int64_t S, int64_t hs, int64_t rs, const float * mask, const float * sinks, float scale,
                             float * out, void * ws, int64_t ws_bytes, hipStream_t s);
+// the 8-bit key-value cache (onpu_kv8.hip); hipErrorInvalidValue past what a grid holds
+hipError_t launch_kv8_write(const Kv8Cache & c, const Kv8Table & t, const void * k, const void * v, int f32, int64_t krs,
+                            int64_t khs, int64_t vrs, int64_t vhs, hipStream_t s);
+hipError_t launch_kv8_read(const Kv8Cache & c, const Kv8Table & t, void * k, void * v, int f32, hipStream_t s);
+int64_t kv8_attn_ws_bytes(int Hq, int D, int Hkv, int nseq, int64_t T, int max_n, int max_len, int window);
+hipError_t launch_kv8_attn(const Kv8Cache & c, const Kv8Table & t, const void * q, int f32, int Hq, int64_t qrs, int64_t qhs,
+                           int max_len, const float * mask, int64_t mld, const float * sinks, int window, float scale,
+                           void * out, void * ws, hipStream_t s);
 hipError_t launch_f32_to_bf16(const float * in, int64_t n, uint16_t * out, hipStream_t s);
 hipError_t launch_moe_act(const float * h, int64_t rows, int64_t Ng, const int32_t * ids, const float * bias, int act,
                           float alpha, float limit, float * o, hipStream_t s);

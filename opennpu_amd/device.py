@@ -5,6 +5,8 @@ stream; every product is computed by the library's HIP kernels.
   QMatrix   one int4 matrix (any format): mv (y = x W^T), argmax (LM head), dequant
   QFfn      routed-expert FFN bank (gate_up + down): route, ffn
   QChain    a fixed sequence of QMatrix GEMVs run in order in one launch (onpu_chain_*)
+  attn_step one decode token of attention over a bf16 / fp32 cache
+  kv8_*     an 8-bit paged key-value cache of one layer: kv8_cache, kv8_write, kv8_read, kv8_attn
 """
 import ctypes as C
 
@@ -236,4 +238,117 @@ def attn_step(q, K, V, mask=None, sinks=None, scale=None, out=None, ws=None):
                                K.stride(0), K.stride(1), None if mask is None else _ptr(mask),
                                None if sinks is None else _ptr(sinks), float(D ** -0.5 if scale is None else scale),
                                _ptr(out), _ptr(ws), ws.numel(), _stream()), "onpu_attn_step_dev")
+    return out
+
+
+def kv8_cache(pages, Hkv, D, device=None):
+    """An empty 8-bit key-value cache of one layer (layout: include/onpu.h): pages of 64 tokens, codes
+    int8 [pages][Hkv][2][64 D] and scales fp32 [pages][Hkv][2]."""
+    import torch
+    return (torch.zeros((pages, Hkv, 2, 64 * D), dtype=torch.int8, device=device or "cuda"),
+            torch.zeros((pages, Hkv, 2), dtype=torch.float32, device=device or "cuda"))
+
+
+def _kv8(codes, scales, table, pos, off, vals, what):
+    """the cache's, table's and row ranges' arguments, checked; vals: (fp32 or bf16 [T][heads][D] tensor, ...)"""
+    import torch
+    pages, Hkv, two, w = codes.shape
+    D = w // 64
+    if codes.dtype != torch.int8 or two != 2 or w % 64 or not codes.is_contiguous():
+        raise ValueError(f"{what}: codes must be int8 [pages][Hkv][2][64 D], contiguous")
+    if scales.dtype != torch.float32 or scales.shape != codes.shape[:3] or not scales.is_contiguous():
+        raise ValueError(f"{what}: scales must be fp32 [pages][Hkv][2], contiguous")
+    nseq, P = table.shape
+    if table.dtype != torch.int32 or (P > 1 and table.stride(1) != 1):
+        raise ValueError(f"{what}: table must be int32 [sequences][P] with rows of unit stride")
+    if pos.dtype != torch.int32 or pos.shape != (nseq,) or not pos.is_contiguous():
+        raise ValueError(f"{what}: positions or lengths must be int32, one per sequence, contiguous")
+    if off is not None and (off.dtype != torch.int32 or off.shape != (nseq + 1,) or not off.is_contiguous()):
+        raise ValueError(f"{what}: off must be int32, one more than the sequences, contiguous")
+    here = torch.cuda.current_device()
+    for t in (codes, scales, table, pos, off) + vals:
+        if t is not None and not (t.is_cuda and t.get_device() == here):
+            raise ValueError(f"{what}: every tensor must be on the current GPU (cuda:{here}), got {t.device}")
+    for t in vals:
+        if t.dim() != 3 or t.shape[2] != D or t.stride(2) != 1 or t.dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"{what}: rows must be fp32 or bf16 [T][heads][{D}] with unit stride in the last dimension")
+    return pages, Hkv, D, nseq, P
+
+
+def _kv8_n(T, nseq, off, max_n, what):
+    """max_n: given, or the rows of each sequence (off None), or the most that one can have"""
+    if off is None:
+        if T % max(nseq, 1):
+            raise ValueError(f"{what}: {T} rows cannot be the same number for each of {nseq} sequences: give off")
+        return T // max(nseq, 1)
+    return T if max_n is None else int(max_n)
+
+
+def kv8_write(codes, scales, k, v, table, pos, off=None, max_n=None):
+    """Quantise k, v (fp32 or bf16 [T][Hkv][D]) into the cache's pages (onpu_kv8_write_dev): sequence i's
+    rows off[i]:off[i + 1] (off None: T / sequences each) go to positions pos[i], pos[i] + 1, ...; max_n: the most
+    rows of one sequence (default: as many as there are)."""
+    import torch
+    L = require_gpu()
+    pages, Hkv, D, nseq, P = _kv8(codes, scales, table, pos, off, (k, v), "kv8_write")
+    if k.shape != v.shape or k.dtype != v.dtype or k.shape[1] != Hkv:
+        raise ValueError("kv8_write: k and v must have the same type and shape [T][Hkv][D]")
+    T = k.shape[0]
+    check(L.onpu_kv8_write_dev(_ptr(codes), _ptr(scales), pages, Hkv, D, _ptr(k), _ptr(v), int(k.dtype == torch.bfloat16),
+                               k.stride(0), k.stride(1), v.stride(0), v.stride(1), _ptr(table), table.stride(0), P,
+                               _ptr(pos), None if off is None else _ptr(off), nseq, T,
+                               _kv8_n(T, nseq, off, max_n, "kv8_write"), _stream()), "kv8_write")
+
+
+def kv8_read(codes, scales, table, pos, rows, off=None, max_n=None, dtype=None, out=None):
+    """The values of positions pos[i], pos[i] + 1, ... of every sequence (onpu_kv8_read_dev): k, v
+    [rows][Hkv][D], bf16 (the default) or fp32; rows in all, off and max_n as kv8_write."""
+    import torch
+    L = require_gpu()
+    pages, Hkv, D, nseq, P = _kv8(codes, scales, table, pos, off, tuple(out or ()), "kv8_read")
+    if out is None:
+        k, v = (torch.empty((rows, Hkv, D), dtype=dtype or torch.bfloat16, device=codes.device) for _ in range(2))
+        if k.dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError("kv8_read: dtype must be fp32 or bf16")
+    else:
+        k, v = out
+        if k.shape != (rows, Hkv, D) or v.shape != k.shape or k.dtype != v.dtype or not (k.is_contiguous() and v.is_contiguous()) \
+                or dtype not in (None, k.dtype):
+            raise ValueError("kv8_read: out must be two contiguous [rows][Hkv][D] tensors of one type")
+    check(L.onpu_kv8_read_dev(_ptr(codes), _ptr(scales), pages, Hkv, D, _ptr(table), table.stride(0), P, _ptr(pos),
+                              None if off is None else _ptr(off), nseq, rows, _kv8_n(rows, nseq, off, max_n, "kv8_read"),
+                              _ptr(k), _ptr(v), int(k.dtype == torch.bfloat16), _stream()), "kv8_read")
+    return k, v
+
+
+def kv8_attn(q, codes, scales, table, lens, off=None, max_n=None, max_len=None, mask=None, sinks=None, window=0, scale=None,
+             out=None, ws=None):
+    """Causal grouped-query attention over the cache (onpu_kv8_attn_dev): q (fp32 or bf16 [T][Hq][D]) are the last
+    rows off[i]:off[i + 1] (off None: T / sequences each) of sequence i's lens[i] cached tokens. max_n, max_len: the most query rows
+    and tokens of one sequence (default: as many as there are, and as the table holds; closer bounds run
+    faster). mask fp32 [sequences][>= max_len] is added to the scores, sinks fp32 [Hq] is a logit per head without a
+    value, window the last positions a query sees (0: all). Returns out [T][Hq][D] in q's type."""
+    import torch
+    L = require_gpu()
+    pages, Hkv, D, nseq, P = _kv8(codes, scales, table, lens, off, (q,) if out is None else (q, out), "kv8_attn")
+    T, Hq = q.shape[0], q.shape[1]
+    n = _kv8_n(T, nseq, off, max_n, "kv8_attn")
+    max_len = 64 * P if max_len is None else int(max_len)
+    if out is None:
+        out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError("kv8_attn: out must be contiguous, of q's shape and type")
+    for t, shape in ((mask, None), (sinks, (Hq,))):
+        if t is not None and (t.dtype != torch.float32 or not t.is_cuda or t.get_device() != q.get_device() or t.stride(-1) != 1
+                              or (t.shape != shape if shape else t.dim() != 2 or t.shape[0] != nseq or t.shape[1] < max_len)):
+            raise ValueError("kv8_attn: mask must be fp32 [sequences][>= max_len], sinks fp32 [Hq], on q's GPU")
+    nb = L.onpu_kv8_attn_ws_bytes(Hq, D, Hkv, nseq, T, n, max_len, window)
+    if nb and ws is None:
+        ws = torch.empty((nb,), dtype=torch.uint8, device=q.device)
+    check(L.onpu_kv8_attn_dev(_ptr(q), int(q.dtype == torch.bfloat16), Hq, q.stride(0), q.stride(1), _ptr(codes),
+                              _ptr(scales), pages, Hkv, D, _ptr(table), table.stride(0), P, _ptr(lens),
+                              None if off is None else _ptr(off), nseq, T, n, max_len, None if mask is None else _ptr(mask),
+                              0 if mask is None else mask.stride(0), None if sinks is None else _ptr(sinks), int(window),
+                              float(D ** -0.5 if scale is None else scale), _ptr(out), None if ws is None else _ptr(ws),
+                              0 if ws is None else ws.nbytes, _stream()), "kv8_attn")
     return out
