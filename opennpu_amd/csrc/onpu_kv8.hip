@@ -159,11 +159,13 @@ struct Kv8AttnArgs {
     const void * q;
     void * out;
     const float * mask, * sinks;
-    float * ws;
+    float * ws;                               // partials of C-token chunks: o [T Hq][nch][D], then (max, sum) [T Hq][nch]
     int64_t qrs, qhs, mld;
     float scale;
-    int Hq, rep, max_len, window;
+    int Hq, rep, max_len, window, f32, C, nch;
 };
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ float wave_max(float v) {
     for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
@@ -173,72 +175,364 @@ __device__ __forceinline__ float wave_sum(float v) {
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
     return v;
 }
+constexpr float LOG2E = 1.44269504088896341f;
 
-// A workgroup per (query row, head); its 4 waves take every fourth page, a lane per token for the scores
-// and a lane per 4 columns for the products, with a running maximum and sum per wave.
-template <bool F32>
-__global__ __launch_bounds__(KT) void k_kv8_attn(Kv8AttnArgs a) {
-    __shared__ float qs[KV8_MAX_D], ps[KT], ml[KT / 64][2], red[KT / 64][KV8_MAX_D];
-    const int D = a.c.D, NC = D / 16, t = threadIdx.x, lane = t & 63, w = t >> 6;
-    const int h = blockIdx.x % a.Hq, j = blockIdx.x / a.Hq, i = blockIdx.y, g = h / a.rep;
+// the larger (or the sum) of x and the lane 32, then 16 away
+template <bool MAX> __device__ __forceinline__ float across_quads(float x) {
+    typedef unsigned u2 __attribute__((ext_vector_type(2)));
+    u2 r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = MAX ? fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)) : __uint_as_float(r.x) + __uint_as_float(r.y);
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return MAX ? fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)) : __uint_as_float(r.x) + __uint_as_float(r.y);
+}
+// the sum over the 4 lanes of a quad permute, the same bits in each
+__device__ __forceinline__ float quad_sum(float x) {
+    x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0xB1, 0xf, 0xf, false));
+    return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x4E, 0xf, 0xf, false));
+}
+
+// Few query rows (a decode token, a verification): bound by the cache's bytes, so the codes go to the int8
+// matrix instructions as they lie in memory, with nothing converted, and the fp32 side is cut into int8
+// instead. A row of q is a fixed-point number of 31 bits below its largest |q| (to 2^-31 of it: more than
+// fp32's own), in four signed bytes; the four are rows 4 h + part of a 16-row operand that holds 4 heads, their
+// integer sums exact. The scores come out as lane (row 4 h + part, quad), token 16 a + 4 quad + c: the
+// order of V's bytes, so the lane's weights, cut the same way (weight e^(x - m) <= 1 to 2^-31), are the other
+// product's operand without a move across lanes. A wave takes every fourth page, K of its next one loading
+// once this one's scores are out, V after its products; waves meet in LDS, chunks in k_kv8_combine.
+// RS sets of 4 rows; NC: chunks of 16 d (D / 16 or more).
+constexpr int SW = KT / 64;                   // waves
+template <int NC, int RS, bool MASK>
+__global__ __launch_bounds__(KT) void k_kv8_step(Kv8AttnArgs a) {
+    constexpr int KS = (NC + 3) / 4, HG = 4 * RS;
+    extern __shared__ __align__(16) float lds[];                 // red [SW][HG][D], ml [SW][HG][2]
+    const int D = a.c.D, nc = D / 16, lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = blockIdx.x % a.c.Hkv, z = blockIdx.x / a.c.Hkv, c = blockIdx.y, i = blockIdx.z;
+    const int quad = lane >> 4, part = lane & 3;
+    const Kv8Rows r = kv8_rows(a.t.off, i, a.t.T, a.t.max_n);
+    const int rows = r.n * a.rep, R0 = z * HG;                   // this group's rows: token R / rep, head g rep + R % rep
+    if (R0 >= rows) return;
+    const int nrow = rows - R0 < HG ? rows - R0 : HG;
+    const int full = a.t.pos[i] < 0 ? 0 : a.t.pos[i], len = full < a.max_len ? full : a.max_len;
+    const int64_t at0 = (int64_t) full - r.n;
+    const Kv8Seen first = kv8_seen(at0 + R0 / a.rep, len, a.window), last = kv8_seen(at0 + (R0 + nrow - 1) / a.rep, len, a.window);
+    const int64_t c0 = (int64_t) c * a.C, c1 = c0 + a.C;
+    const int lo = first.lo > c0 ? first.lo : (int) (c0 < last.hi ? c0 : last.hi), hi = last.hi < c1 ? last.hi : (int) c1;
+    if (a.nch > 1 && lo >= hi) return;
+    const int pend = (hi + KV8_PAGE - 1) / KV8_PAGE;
+    const int32_t * tab = a.t.table + i * a.t.tld;
+    const float nan = __uint_as_float(0x7fc00000u);
+
+    // q, 16 values of a lane's row and step
+    float q[RS][KS][16];
+    int rlo[RS], rhi[RS];
+#pragma unroll
+    for (int k = 0; k < RS; k++) {
+        const int rr = 4 * k + ((lane & 15) >> 2) < nrow ? 4 * k + ((lane & 15) >> 2) : nrow - 1;
+        const int R = R0 + rr, j = R / a.rep, h = g * a.rep + (R - j * a.rep);
+        const Kv8Seen s = kv8_seen(at0 + j, len, a.window);
+        rlo[k] = s.lo;
+        rhi[k] = s.hi;
+        const int64_t base = (r.row + j) * a.qrs + h * a.qhs;
+#pragma unroll
+        for (int s2 = 0; s2 < KS; s2++) {
+            const int d = 64 * s2 + 16 * quad;
+            if (a.f32) load16<true>(a.q, base + (d < D ? d : 0), q[k][s2]);
+            else load16<false>(a.q, base + (d < D ? d : 0), q[k][s2]);
+            if (d >= D)
+#pragma unroll
+                for (int e = 0; e < 16; e++) q[k][s2][e] = 0.f;
+        }
+    }
+    uint4 kr[4][KS], vr[NC];
+    float sk, sv;
+    auto page_base = [&](int id) { return a.c.codes + ((int64_t) (id < 0 ? 0 : id) * a.c.Hkv + g) * 2 * KV8_PAGE * D; };
+    auto load_k = [&](int id) {               // (steps past D meet zeros of q; they read on into V's codes)
+        const int8_t * p = page_base(id) + 16 * lane;
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int s = 0; s < KS; s++) kr[t][s] = *(const uint4 *) (p + t * nc * 256 + s * 1024);
+    };
+    auto load_v = [&](int id) {               // (chunks past D re-read the last: not stored)
+        const int8_t * p = page_base(id) + KV8_PAGE * D + 16 * lane;
+#pragma unroll
+        for (int n = 0; n < NC; n++) vr[n] = *(const uint4 *) (p + (n < nc ? n : nc - 1) * 1024);
+    };
+    auto load_s = [&](int id) {
+        const float * p = a.c.scales + ((int64_t) (id < 0 ? 0 : id) * a.c.Hkv + g) * 2;
+        const bool bad = id < 0 || full > a.max_len;
+        sk = bad ? nan : p[0];
+        sv = bad ? nan : p[1];
+    };
+    int pg = lo / KV8_PAGE + w;
+    if (pg < pend) {
+        const int id = kv8_page(tab, pg, a.t.P, a.c.pages);
+        load_k(id);
+        load_v(id);
+        load_s(id);
+    }
+    // the rows' bytes
+    const uint32_t b = 3 - part, flip = part ? 0x80808080u : 0u;
+    const uint32_t sel01 = 0x0c0c0000u | (4 + b) << 8 | b, sel23 = 0x00000c0cu | (4 + b) << 24 | b << 16;
+    auto cut = [&](uint32_t y0, uint32_t y1, uint32_t y2, uint32_t y3) {           // byte `part` of four fixed-point numbers
+        constexpr uint32_t bias = 0x00808080u;
+        return (__builtin_amdgcn_perm(y1 + bias, y0 + bias, sel01) | __builtin_amdgcn_perm(y3 + bias, y2 + bias, sel23)) ^ flip;
+    };
+    i32x4 qa[RS][KS];
+    float rowf[RS];
+#pragma unroll
+    for (int k = 0; k < RS; k++) {
+        uint32_t mq = 0;
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) mq = max(mq, __float_as_uint(q[k][s][e]) & 0x7fffffffu);
+        float big = __uint_as_float(mq);                         // NaN (as a number the largest) has to win
+        mq = max(mq, (uint32_t) __shfl_xor((int) mq, 16));
+        mq = max(mq, (uint32_t) __shfl_xor((int) mq, 32));
+        big = __uint_as_float(mq);
+        const int e2 = mq >= 0x7f800000u ? 0 : __builtin_amdgcn_frexp_expf(big);     // big < 2^e2
+        rowf[k] = mq >= 0x7f800000u ? nan : ldexpf(MASK ? a.scale : a.scale * LOG2E, e2 - 30);
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                uint32_t y[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[e] = (uint32_t) (int) rintf(ldexpf(q[k][s][4 * u + e], 30 - e2));
+                qa[k][s][u] = cut(y[0], y[1], y[2], y[3]);
+            }
+    }
+    const float pw = __uint_as_float((127u + 8 * b) << 23);      // 256^(3 - part)
+    float m[RS], l[RS], acc[RS][NC];
+#pragma unroll
+    for (int k = 0; k < RS; k++) {
+        m[k] = -__builtin_inff();
+        l[k] = 0.f;
+#pragma unroll
+        for (int n = 0; n < NC; n++) acc[k][n] = 0.f;
+    }
+    for (; pg < pend; pg += SW) {
+        const int t0 = pg * KV8_PAGE, next = pg + SW < pend ? kv8_page(tab, pg + SW, a.t.P, a.c.pages) : -1;
+        const float skc = sk, svc = sv;
+        i32x4 sc[RS][4];
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int k = 0; k < RS; k++) {
+                i32x4 d = {0, 0, 0, 0};
+#pragma unroll
+                for (int s = 0; s < KS; s++)
+                    d = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, kr[t][s]), qa[k][s], d, 0, 0, 0);
+                sc[k][t] = d;
+            }
+        if (pg + SW < pend) { load_k(next); load_s(next); }
+        float4 mk[4];
+        if (MASK) {
+            const __amdgpu_buffer_rsrc_t mr = __builtin_amdgcn_make_buffer_rsrc(
+                (void *) (a.mask + i * a.mld + t0), (short) 0, 4 * (hi - t0 < KV8_PAGE ? hi - t0 : KV8_PAGE), 0x00020000);
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                mk[t].x = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(mr, 4 * (16 * t + 4 * quad), 0, 0));
+                mk[t].y = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(mr, 4 * (16 * t + 4 * quad) + 4, 0, 0));
+                mk[t].z = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(mr, 4 * (16 * t + 4 * quad) + 8, 0, 0));
+                mk[t].w = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(mr, 4 * (16 * t + 4 * quad) + 12, 0, 0));
+            }
+        }
+        const bool edge = t0 < last.lo || t0 + KV8_PAGE > first.hi || t0 < lo || t0 + KV8_PAGE > hi;
+        i32x4 pa[RS];
+        float al[RS];
+        bool up = false;
+#pragma unroll
+        for (int k = 0; k < RS; k++) {
+            const float f = rowf[k] * skc;
+            float x[16];
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float y = quad_sum((float) sc[k][t][e] * pw) * f;
+                    if (MASK) y += e == 0 ? mk[t].x : (e == 1 ? mk[t].y : (e == 2 ? mk[t].z : mk[t].w));
+                    x[4 * t + e] = y;
+                }
+            if (edge) {
+                const int l0 = (rlo[k] > lo ? rlo[k] : lo) - t0 - 4 * quad, h0 = (rhi[k] < hi ? rhi[k] : hi) - t0 - 4 * quad;
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const int n = 16 * (e >> 2) + (e & 3);
+                    x[e] = n >= l0 && n < h0 ? x[e] : -__builtin_inff();
+                }
+            }
+            float mx = x[0];
+#pragma unroll
+            for (int e = 1; e < 16; e++) mx = fmaxf(mx, x[e]);
+            mx = fmaxf(m[k], across_quads<true>(mx));
+            const float base = mx == -__builtin_inff() ? 0.f : mx;
+            al[k] = m[k] == mx ? 1.f : __builtin_amdgcn_exp2f(MASK ? (m[k] - base) * LOG2E : m[k] - base);
+            up = up || m[k] != mx;
+            m[k] = mx;
+            float sum = 0.f;
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                uint32_t y[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float p = __builtin_amdgcn_exp2f(MASK ? (x[4 * t + e] - base) * LOG2E : x[4 * t + e] - base);
+                    sum += p;
+                    y[e] = (uint32_t) (int) fmaf(p, 1073741824.f, 0.5f);
+                }
+                pa[k][t] = cut(y[0], y[1], y[2], y[3]);
+            }
+            l[k] = fmaf(l[k], al[k], sum);
+        }
+        if (__any(up)) {
+#pragma unroll
+            for (int k = 0; k < RS; k++) {
+                const float f = __shfl(al[k], 4 * quad);         // of the head whose o this lane holds
+#pragma unroll
+                for (int n = 0; n < NC; n++) acc[k][n] *= f;
+            }
+        }
+        float fh[RS], fl[RS];                                    // the value of a step of o's upper and lower bytes
+#pragma unroll
+        for (int k = 0; k < RS; k++) {
+            fh[k] = svc * 6.103515625e-05f;                      // 2^-14, 2^-30
+            fl[k] = svc * 9.31322574615478515625e-10f;
+            if (svc != svc && !__shfl((int) (rlo[k] < t0 + KV8_PAGE && rhi[k] > t0), 4 * quad)) fh[k] = fl[k] = 0.f;
+        }                                                        // (NaN only where a row sees the page)
+#pragma unroll
+        for (int n = 0; n < NC; n++)
+#pragma unroll
+            for (int k = 0; k < RS; k++) {
+                const i32x4 d = __builtin_amdgcn_mfma_i32_16x16x64_i8(pa[k], __builtin_bit_cast(i32x4, vr[n]), (i32x4){0, 0, 0, 0}, 0, 0, 0);
+                acc[k][n] = fmaf((float) ((d[0] << 8) + d[1]), fh[k], acc[k][n]);
+                acc[k][n] = fmaf((float) ((d[2] << 8) + d[3]), fl[k], acc[k][n]);
+            }
+        if (pg + SW < pend) load_v(next);
+    }
+    // the waves' rows meet
+    float * red = lds, * ml = lds + SW * HG * D;
+#pragma unroll
+    for (int k = 0; k < RS; k++) {
+        const float sum = across_quads<false>(l[k]);
+        if (part == 0 && quad == 0) {
+            ml[(w * HG + 4 * k + (lane >> 2)) * 2] = m[k];
+            ml[(w * HG + 4 * k + (lane >> 2)) * 2 + 1] = sum;
+        }
+#pragma unroll
+        for (int n = 0; n < NC; n++)
+            if (n < nc) red[(w * HG + 4 * k + quad) * D + 16 * n + (lane & 15)] = acc[k][n];
+    }
+    __syncthreads();
+    const float unit = MASK ? LOG2E : 1.f;                       // (maxima are in powers of 2 without a mask)
+    float * wml = a.ws + a.t.T * a.Hq * a.nch * D;
+    for (int u = threadIdx.x; u < nrow * D; u += KT) {
+        const int rr = u / D, d = u - rr * D;
+        const int R = R0 + rr, j = R / a.rep, h = g * a.rep + (R - j * a.rep);
+        const int64_t o = (r.row + j) * a.Hq + h;
+        const float sink = a.sinks && a.nch == 1 ? a.sinks[h] * (MASK ? 1.f : LOG2E) : -__builtin_inff();
+        float M = sink, L = 0.f, y = 0.f;
+#pragma unroll
+        for (int k = 0; k < SW; k++) M = fmaxf(M, ml[(k * HG + rr) * 2]);
+        const float base = M == -__builtin_inff() ? 0.f : M;
+#pragma unroll
+        for (int k = 0; k < SW; k++) {
+            const float f = __builtin_amdgcn_exp2f((ml[(k * HG + rr) * 2] - base) * unit);
+            L = fmaf(f, ml[(k * HG + rr) * 2 + 1], L);
+            if (ml[(k * HG + rr) * 2 + 1] != ml[(k * HG + rr) * 2 + 1]) L = nan;     // no score but NaN
+            y = fmaf(f, red[(k * HG + rr) * D + d], y);
+        }
+        if (a.nch == 1) {
+            if (a.sinks) L += __builtin_amdgcn_exp2f((sink - base) * unit);
+            y = L == 0.f ? 0.f : y / L;
+            if (a.f32) ((float *) a.out)[o * D + d] = y;
+            else ((uint16_t *) a.out)[o * D + d] = f32_to_bf16(y);
+        } else {
+            a.ws[(o * a.nch + c) * D + d] = y;
+            if (d == 0) {
+                wml[(o * a.nch + c) * 2] = M;
+                wml[(o * a.nch + c) * 2 + 1] = L;
+            }
+        }
+    }
+}
+
+// The chunks of a row joined: a workgroup per (row, head). A wave finds the largest maximum and the
+// weights, a chunk a lane; every thread then adds its column over its share of the chunks.
+__global__ __launch_bounds__(KT) void k_kv8_combine(Kv8AttnArgs a) {
+    __shared__ float sred[KT], sw[SW][64], sden[SW];
+    const int D = a.c.D, h = blockIdx.x % a.Hq, j = blockIdx.x / a.Hq, i = blockIdx.y, t = threadIdx.x, lane = t & 63, w = t >> 6;
     const Kv8Rows r = kv8_rows(a.t.off, i, a.t.T, a.t.max_n);
     if (j >= r.n) return;
-    const int64_t row = r.row + j;
     const int full = a.t.pos[i] < 0 ? 0 : a.t.pos[i], len = full < a.max_len ? full : a.max_len;
-    const Kv8Seen seen = kv8_seen((int64_t) full - r.n + j, len, a.window);
-    for (int d = t; d < D; d += KT)
-        qs[d] = F32 ? ((const float *) a.q)[row * a.qrs + h * a.qhs + d] : bf16_to_f32(((const uint16_t *) a.q)[row * a.qrs + h * a.qhs + d]);
-    __syncthreads();
-    float m = -__builtin_inff(), l = 0.f, o[4] = {0, 0, 0, 0};
-    for (int pg = seen.lo / KV8_PAGE + w; pg * KV8_PAGE < seen.hi; pg += KT / 64) {
-        const int id = kv8_page(a.t.table + i * a.t.tld, pg, a.t.P, a.c.pages), token = pg * KV8_PAGE + lane;
-        const int8_t * kc = a.c.codes + ((int64_t) (id < 0 ? 0 : id) * a.c.Hkv + g) * 2 * KV8_PAGE * D, * vc = kc + KV8_PAGE * D;
-        const float * sc = a.c.scales + ((int64_t) (id < 0 ? 0 : id) * a.c.Hkv + g) * 2;
-        const bool bad = id < 0 || full > a.max_len;
-        const float sk = bad ? __uint_as_float(0x7fc00000u) : sc[0], sv = bad ? __uint_as_float(0x7fc00000u) : sc[1];
-        float x = 0.f;
-        for (int d = 0; d < D; d++) x += qs[d] * kc[kv8_k_at(D, lane, d)];
-        x = x * (sk * a.scale);
-        const bool see = token >= seen.lo && token < seen.hi;
-        if (a.mask && see) x += a.mask[i * a.mld + token];
-        if (!see) x = -__builtin_inff();
-        const float mn = fmaxf(m, wave_max(x)), base = mn == -__builtin_inff() ? 0.f : mn;
-        const float p = x == -__builtin_inff() ? 0.f : expf(x - base), f = m == -__builtin_inff() ? 0.f : expf(m - base);
-        l = l * f + p;
-        ps[t] = p;
-        __builtin_amdgcn_wave_barrier();
-        for (int k = 0; k < 4; k++) {
-            const int d = lane + 64 * k;
-            if (d >= D) continue;
-            float y = 0.f;
-            for (int n = 0; n < KV8_PAGE; n++) y += ps[64 * w + n] * vc[kv8_v_at(D, n, d)];
-            o[k] = o[k] * f + y * sv;
-        }
-        __builtin_amdgcn_wave_barrier();
-        m = mn;
-    }
-    l = wave_sum(l);
-    if (lane == 0) { ml[w][0] = m; ml[w][1] = l; }
-    for (int k = 0; k < 4; k++)
-        if (lane + 64 * k < D) red[w][lane + 64 * k] = o[k];
-    __syncthreads();
-    float M = a.sinks ? a.sinks[h] : -__builtin_inff(), L = 0.f;
-    for (int k = 0; k < KT / 64; k++) M = fmaxf(M, ml[k][0]);
+    const Kv8Seen s = kv8_seen((int64_t) full - r.n + j, len, a.window);
+    const int ca = s.lo / a.C, cb = s.hi > s.lo ? (s.hi - 1) / a.C + 1 : ca;   // the chunks that this row sees
+    const int64_t o = (r.row + j) * a.Hq + h;
+    const float * wo = a.ws + o * a.nch * D, * wml = a.ws + a.t.T * a.Hq * a.nch * D + o * a.nch * 2;
+    // (maxima are in powers of 2 without a mask, in powers of e with one: its lowest value has to fit)
+    const float unit = a.mask ? LOG2E : 1.f, sink = a.sinks ? a.sinks[h] * (a.mask ? 1.f : LOG2E) : -__builtin_inff();
+    float M = sink;
+    for (int c = ca + lane; c < cb; c += 64) M = fmaxf(M, wml[2 * c]);
+    M = wave_max(M);
     const float base = M == -__builtin_inff() ? 0.f : M;
-    float f[KT / 64];
-    for (int k = 0; k < KT / 64; k++) {
-        f[k] = ml[k][0] == -__builtin_inff() ? (ml[k][1] != 0.f ? ml[k][1] : 0.f) : expf(ml[k][0] - base);    // (NaN stays)
-        L += f[k] * ml[k][1];
+    float den = 0.f, y = 0.f;
+    const int DP = D <= 64 ? 64 : (D <= 128 ? 128 : 256), G = KT / DP, d = t % DP, gr = t / DP;
+    for (int b = ca; b < cb; b += 64) {
+        const int c = b + lane;
+        const float f = c < cb ? __builtin_amdgcn_exp2f((wml[2 * c] - base) * unit) : 0.f;
+        if (c < cb) {
+            const float lc = wml[2 * c + 1];
+            den = lc != lc ? lc : fmaf(f, lc, den);
+        }
+        sw[w][lane] = f;
+        __builtin_amdgcn_wave_barrier();
+        const int n = cb - b < 64 ? cb - b : 64;
+        if (d < D)
+            for (int k = gr; k < n; k += G) y = fmaf(sw[w][k], wo[(int64_t) (b + k) * D + d], y);
+        __builtin_amdgcn_wave_barrier();
     }
-    if (a.sinks) L += expf(a.sinks[h] - base);
-    for (int d = t; d < D; d += KT) {
-        float y = 0.f;
-        for (int k = 0; k < KT / 64; k++) y += f[k] == 0.f ? 0.f : f[k] * red[k][d];
-        y = L == 0.f ? 0.f : y / L;
-        const int64_t at = (row * a.Hq + h) * D + d;
-        if (F32) ((float *) a.out)[at] = y;
-        else ((uint16_t *) a.out)[at] = f32_to_bf16(y);
+    den = wave_sum(den) + (a.sinks ? __builtin_amdgcn_exp2f((sink - base) * unit) : 0.f);
+    sred[t] = y;
+    __syncthreads();
+    if (t < D && gr == 0) {
+        for (int k = 1; k < G; k++) y += sred[k * DP + t];
+        y = den == 0.f ? 0.f : y / den;
+        if (a.f32) ((float *) a.out)[o * D + t] = y;
+        else ((uint16_t *) a.out)[o * D + t] = f32_to_bf16(y);
     }
+}
+
+struct AttnPlan { int RS, ngrp, C, nch; };
+
+AttnPlan attn_plan(int Hq, int Hkv, int nseq, int max_n, int max_len, int window) {
+    AttnPlan p;
+    const int64_t rows = (int64_t) max_n * (Hq / Hkv);
+    p.RS = rows <= 4 ? 1 : (rows <= 8 ? 2 : 4);
+    p.ngrp = (int) ((rows + 4 * p.RS - 1) / (4 * p.RS));
+    // chunks of whole rounds of the waves
+    const int64_t round = SW * KV8_PAGE, wgs = (int64_t) Hkv * p.ngrp * nseq;
+    int64_t nch = (1024 + wgs - 1) / wgs, most = (max_len + round - 1) / round;
+    if (nch > most) nch = most;
+    int64_t C = (max_len + nch - 1) / nch;
+    C = (C + round - 1) / round * round;
+    p.C = (int) (C > (1 << 30) ? 1 << 30 : C);
+    p.nch = (int) ((max_len + (int64_t) p.C - 1) / p.C);
+    return p;
+}
+
+template <int NC, int RS> hipError_t run_step(const Kv8AttnArgs & a, const AttnPlan & p, hipStream_t s) {
+    const dim3 grid((unsigned) (a.c.Hkv * p.ngrp), (unsigned) p.nch, (unsigned) a.t.nseq);
+    const size_t lds = sizeof(float) * SW * 4 * RS * (a.c.D + 2);
+    if (a.mask) k_kv8_step<NC, RS, true><<<grid, KT, lds, s>>>(a);
+    else k_kv8_step<NC, RS, false><<<grid, KT, lds, s>>>(a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.nch == 1) return e;
+    k_kv8_combine<<<dim3((unsigned) (a.Hq * a.t.max_n), (unsigned) a.t.nseq), KT, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+template <int NC> hipError_t run_step_rs(const Kv8AttnArgs & a, const AttnPlan & p, hipStream_t s) {
+    return p.RS == 1 ? run_step<NC, 1>(a, p, s) : (p.RS == 2 ? run_step<NC, 2>(a, p, s) : run_step<NC, 4>(a, p, s));
 }
 
 }  // namespace
@@ -265,15 +559,19 @@ hipError_t launch_kv8_read(const Kv8Cache & c, const Kv8Table & t, void * k, voi
     return hipGetLastError();
 }
 
-int64_t kv8_attn_ws_bytes(int, int, int, int, int64_t, int, int, int) { return 0; }
+int64_t kv8_attn_ws_bytes(int Hq, int D, int Hkv, int nseq, int64_t T, int max_n, int max_len, int window) {
+    const AttnPlan p = attn_plan(Hq, Hkv, nseq, max_n, max_len, window);
+    return p.nch == 1 ? 0 : T * Hq * p.nch * (D + 2) * (int64_t) sizeof(float);
+}
 
 hipError_t launch_kv8_attn(const Kv8Cache & c, const Kv8Table & t, const void * q, int f32, int Hq, int64_t qrs, int64_t qhs,
                            int max_len, const float * mask, int64_t mld, const float * sinks, int window, float scale,
                            void * out, void * ws, hipStream_t s) {
-    Kv8AttnArgs a{c, t, q, out, mask, sinks, (float *) ws, qrs, qhs, mld, scale, Hq, Hq / c.Hkv, max_len, window};
-    if (!grid_fits((int64_t) Hq * t.max_n, t.nseq)) return hipErrorInvalidValue;
-    const dim3 grid((unsigned) (Hq * t.max_n), (unsigned) t.nseq);
-    if (f32) k_kv8_attn<true><<<grid, KT, 0, s>>>(a);
-    else k_kv8_attn<false><<<grid, KT, 0, s>>>(a);
-    return hipGetLastError();
+    const AttnPlan p = attn_plan(Hq, c.Hkv, t.nseq, t.max_n, max_len, window);
+    Kv8AttnArgs a{c, t, q, out, mask, sinks, (float *) ws, qrs, qhs, mld, scale, Hq, Hq / c.Hkv, max_len, window, f32, p.C, p.nch};
+    if (!grid_fits((int64_t) Hq * t.max_n, t.nseq) || !grid_fits((int64_t) c.Hkv * p.ngrp, t.nseq) || p.nch > 65535)
+        return hipErrorInvalidValue;
+    const int nc = c.D / 16;
+    return nc <= 4 ? run_step_rs<4>(a, p, s) : (nc <= 6 ? run_step_rs<6>(a, p, s) : (nc <= 8 ? run_step_rs<8>(a, p, s) :
+           (nc <= 12 ? run_step_rs<12>(a, p, s) : run_step_rs<16>(a, p, s))));
 }
