@@ -295,7 +295,7 @@ int onpu_kv8_read_dev(const void * codes, const float * scales, int64_t pages, i
  * for which no position has a weight gives zeros. max_len: at least the longest of lens; a sequence
  * with more gives NaN. ws: onpu_kv8_attn_ws_bytes bytes (0: none needed), 16-byte aligned; calls in
  * flight together need their own. */
-int64_t onpu_kv8_attn_ws_bytes(int Hq, int D, int Hkv, int nseq, int64_t T, int max_n, int max_len, int window);
+int64_t onpu_kv8_attn_ws_bytes(int q_bf16, int Hq, int D, int Hkv, int nseq, int64_t T, int max_n, int max_len, int window);
 int onpu_kv8_attn_dev(const void * q, int q_bf16, int Hq, int64_t qrs, int64_t qhs, const void * codes, const float * scales,
                       int64_t pages, int Hkv, int D, const int32_t * table, int64_t tld, int P, const int32_t * lens,
                       const int32_t * off, int nseq, int64_t T, int max_n, int max_len, const float * mask, int64_t mld,

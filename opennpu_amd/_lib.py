@@ -94,7 +94,7 @@ def _declare(lib):
         "onpu_kv8_write_dev": (I32, [P, P, I64, I32, I32, P, P, I32, I64, I64, I64, I64, P, I64, I32, P, P, I32, I64, I32,
                                      P]),
         "onpu_kv8_read_dev": (I32, [P, P, I64, I32, I32, P, I64, I32, P, P, I32, I64, I32, P, P, I32, P]),
-        "onpu_kv8_attn_ws_bytes": (I64, [I32, I32, I32, I32, I64, I32, I32, I32]),
+        "onpu_kv8_attn_ws_bytes": (I64, [I32, I32, I32, I32, I32, I64, I32, I32, I32]),
         "onpu_kv8_attn_dev": (I32, [P, I32, I32, I64, I64, P, P, I64, I32, I32, P, I64, I32, P, P, I32, I64, I32, I32, P,
                                     I64, P, I32, C.c_float, P, P, I64, P]),
         "onpu_chain_new": (P, [C.POINTER(P), C.POINTER(P), C.POINTER(P), I32, I64, I32]),

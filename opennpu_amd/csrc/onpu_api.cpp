@@ -1967,9 +1967,9 @@ int onpu_kv8_read_dev(const void * codes, const float * scales, int64_t pages, i
                     launch_kv8_read(c, t, k, v, !kv_bf16, (hipStream_t) stream));
 }
 
-int64_t onpu_kv8_attn_ws_bytes(int Hq, int D, int Hkv, int nseq, int64_t T, int max_n, int max_len, int window) {
+int64_t onpu_kv8_attn_ws_bytes(int q_bf16, int Hq, int D, int Hkv, int nseq, int64_t T, int max_n, int max_len, int window) {
     if (Hq <= 0 || D <= 0 || Hkv <= 0 || Hq % Hkv || nseq <= 0 || T <= 0 || max_n <= 0 || max_len <= 0) return 0;
-    return kv8_attn_ws_bytes(Hq, D, Hkv, nseq, T, max_n, max_len, window);
+    return kv8_attn_ws_bytes(!q_bf16, Hq, D, Hkv, nseq, T, max_n, max_len, window);
 }
 
 int onpu_kv8_attn_dev(const void * q, int q_bf16, int Hq, int64_t qrs, int64_t qhs, const void * codes, const float * scales,
@@ -1990,7 +1990,7 @@ int onpu_kv8_attn_dev(const void * q, int q_bf16, int Hq, int64_t qrs, int64_t q
         set_err("onpu_kv8_attn_dev: needs q and out fp32 or bf16, rows and heads on 16 bytes");
         return -1;
     }
-    const int64_t need = kv8_attn_ws_bytes(Hq, D, Hkv, nseq, T, max_n, max_len, window);
+    const int64_t need = kv8_attn_ws_bytes(!q_bf16, Hq, D, Hkv, nseq, T, max_n, max_len, window);
     if (need > 0 && (!ws || ws_bytes < need || (uintptr_t) ws % 16)) {
         set_err("onpu_kv8_attn_dev: needs a 16-byte aligned workspace of onpu_kv8_attn_ws_bytes");
         return -1;

@@ -162,7 +162,7 @@ struct Kv8AttnArgs {
     float * ws;                               // partials of C-token chunks: o [T Hq][nch][D], then (max, sum) [T Hq][nch]
     int64_t qrs, qhs, mld;
     float scale;
-    int Hq, rep, max_len, window, f32, C, nch;
+    int Hq, rep, max_len, window, f32, C, nch, fold;
 };
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -457,6 +457,310 @@ __global__ __launch_bounds__(KT) void k_kv8_step(Kv8AttnArgs a) {
     }
 }
 
+// Many query rows (prompts): bound by the matrix cores and, nearly as much, by the softmax's vector work.
+// A workgroup takes 128 rows (token, head of the kv head g), 32 a wave, and goes through the pages
+// that they see; a page's codes become fp16 (exact) in LDS once for its 4 waves, in the order that the
+// matrix instructions take them, two pages deep with the next one's codes in registers. A wave forms
+// S^T = K q^T: lane (row n, half) then holds tokens 32 T + 8 i + 4 half + c, which, V's tokens being taken in
+// the same order, is the operand of O^T = V^T P^T without a move across lanes. Rounding: q (bf16) is
+// exact in fp16 after scaling its row by a power of two (to 2^-32 of the largest); the weights are
+// rounded to fp16 (half a step 2^-12 of each, and the row's sum adds the rounded ones), below the
+// output's bf16; sums, maxima and o are fp32. The V scale rides on the weights, relative to a power of
+// two 2^eref that follows it; a row's reference maximum moves only when a score passes it by 2^3.
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+// four codes -> fp16, exactly: 1024 + (code + 128) by its bits, less 1152
+__device__ __forceinline__ void codes_f16(uint32_t u, uint32_t & lo, uint32_t & hi) {
+    u ^= 0x80808080u;
+    const f16x2 k = {(_Float16) -1152.f, (_Float16) -1152.f};
+    lo = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) + k);
+    hi = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + k);
+}
+
+constexpr int TR = 32 * SW;                   // rows of a workgroup
+template <int NC, bool MASK>
+__global__ __launch_bounds__(KT, NC <= 8 ? 2 : 1) void k_kv8_tile(Kv8AttnArgs a) {
+    constexpr int NU = NC / 2, ND = NC / 2, FRAGS = 4 * NC;      // load units of a wave, d tiles of 32, KiB of a page
+    extern __shared__ __align__(16) uint4 page[];                // [2][FRAGS][64]
+    const int D = a.c.D, nc = D / 16, lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = blockIdx.y, i = blockIdx.z, half = lane >> 5, n31 = lane & 31;
+    const int g = blockIdx.x % a.c.Hkv;
+    int z = blockIdx.x / a.c.Hkv;
+    const Kv8Rows r = kv8_rows(a.t.off, i, a.t.T, a.t.max_n);
+    const int rows = r.n * a.rep, ngrp = (rows + TR - 1) / TR;
+    if (z >= ngrp) return;
+    // the longest first; with no more workgroups than run at once, the second half the shortest first, so that
+    // what two workgroups of a CU have adds to the same
+    z = a.fold && z >= ngrp / 2 ? z - ngrp / 2 : ngrp - 1 - z;
+    const int R0 = z * TR, nrow = rows - R0 < TR ? rows - R0 : TR;
+    const int full = a.t.pos[i] < 0 ? 0 : a.t.pos[i], len = full < a.max_len ? full : a.max_len;
+    const int64_t at0 = (int64_t) full - r.n;
+    const Kv8Seen first = kv8_seen(at0 + R0 / a.rep, len, a.window), last = kv8_seen(at0 + (R0 + nrow - 1) / a.rep, len, a.window);
+    const int64_t c0 = (int64_t) c * a.C, c1 = c0 + a.C;
+    const int lo = first.lo > c0 ? first.lo : (int) (c0 < last.hi ? c0 : last.hi), hi = last.hi < c1 ? last.hi : (int) c1;
+    if (a.nch > 1 && lo >= hi) return;
+    const int pbeg = lo / KV8_PAGE, pend = (hi + KV8_PAGE - 1) / KV8_PAGE;
+    const int32_t * tab = a.t.table + i * a.t.tld;
+    const float nan = __uint_as_float(0x7fc00000u), inf = __builtin_inff();
+
+    // this wave's share of a page: where each unit's 16 bytes are, and the fragments that they make
+    int src[NU], dst[NU][2];
+#pragma unroll
+    for (int u = 0; u < NU; u++) {
+        const int k = w + SW * u;
+        if (k < NC) {                                            // K: tokens 32 T + n31, chunk 2 s + half
+            const int T = k / (NC / 2), s2 = k % (NC / 2), ch = 2 * s2 + half < nc ? 2 * s2 + half : nc - 1;
+            src[u] = ((2 * T + (n31 >> 4)) * nc + ch) * 256 + (lane & 15) * 16;
+            dst[u][0] = (T * NC + 2 * s2) * 64 + lane;
+            dst[u][1] = dst[u][0] + 64;
+        } else {                                                 // V: d 32 dt + n31, tokens' quad 2 v + half
+            const int dt = (k - NC) >> 1, v = (k - NC) & 1, ch = 2 * dt + (n31 >> 4) < nc ? 2 * dt + (n31 >> 4) : nc - 1;
+            src[u] = KV8_PAGE * D + ch * 1024 + (2 * v + half) * 256 + (lane & 15) * 16;
+            dst[u][0] = (2 * NC + dt * 4 + v) * 64 + lane;
+            dst[u][1] = dst[u][0] + 128;
+        }
+    }
+    uint4 raw[NU];
+    auto load = [&](int id) {
+        const int8_t * p = a.c.codes + ((int64_t) (id < 0 ? 0 : id) * a.c.Hkv + g) * 2 * KV8_PAGE * D;
+#pragma unroll
+        for (int u = 0; u < NU; u++) raw[u] = *(const uint4 *) (p + src[u]);
+    };
+    auto store = [&](uint4 * to) {
+#pragma unroll
+        for (int u = 0; u < NU; u++) {
+            uint4 x, y;
+            codes_f16(raw[u].x, x.x, x.y);
+            codes_f16(raw[u].y, x.z, x.w);
+            codes_f16(raw[u].z, y.x, y.y);
+            codes_f16(raw[u].w, y.z, y.w);
+            to[dst[u][0]] = x;
+            to[dst[u][1]] = y;
+        }
+    };
+    auto page_id = [&](int p) { return p < pend ? kv8_page(tab, p, a.t.P, a.c.pages) : 0; };
+    auto scale_of = [&](int id, float & k, float & v) {
+        const float * p = a.c.scales + ((int64_t) (id < 0 ? 0 : id) * a.c.Hkv + g) * 2;
+        const bool bad = id < 0 || full > a.max_len;
+        k = bad ? nan : p[0];
+        v = bad ? nan : p[1];
+    };
+
+    // this lane's row
+    const int rr = w * 32 + n31 < nrow ? w * 32 + n31 : nrow - 1, j = (R0 + rr) / a.rep, h = g * a.rep + (R0 + rr - j * a.rep);
+    const Kv8Seen mine = kv8_seen(at0 + j, len, a.window);
+    const bool live = w * 32 < nrow;                             // a wave behind the last row only loads
+    const int wl = live ? w * 32 : nrow - 1, wh = w * 32 + 31 < nrow ? w * 32 + 31 : nrow - 1;
+    const Kv8Seen wfirst = kv8_seen(at0 + (R0 + wl) / a.rep, len, a.window), wlast = kv8_seen(at0 + (R0 + wh) / a.rep, len, a.window);
+    f16x8 q[NC];
+    float rowf;
+    {
+        const uint16_t * p = (const uint16_t *) a.q + (r.row + j) * a.qrs + h * a.qhs;
+        uint4 u[NC];
+        uint32_t mq = 0;
+#pragma unroll
+        for (int s2 = 0; s2 < NC / 2; s2++)
+#pragma unroll
+            for (int v = 0; v < 2; v++) {
+                const int d = 16 * (2 * s2 + half) + 8 * v;
+                uint4 x = *(const uint4 *) (p + (d < D ? d : 0));
+                if (d >= D) x = make_uint4(0, 0, 0, 0);
+                u[2 * s2 + v] = x;
+                mq = max(mq, max(max(x.x & 0x7fff0000u, x.y & 0x7fff0000u), max(x.z & 0x7fff0000u, x.w & 0x7fff0000u)));
+                mq = max(mq, max(max(x.x << 16 & 0x7fff0000u, x.y << 16 & 0x7fff0000u), max(x.z << 16 & 0x7fff0000u, x.w << 16 & 0x7fff0000u)));
+            }
+        mq = max(mq, (uint32_t) __shfl_xor((int) mq, 32));
+        const int e2 = mq >= 0x7f800000u ? 0 : __builtin_amdgcn_frexp_expf(__uint_as_float(mq));     // the largest < 2^e2, to 2^8
+        rowf = mq >= 0x7f800000u ? nan : ldexpf(fabsf(a.scale) * (MASK ? 1.f : LOG2E), e2 - 8);
+        const float sign = a.scale < 0.f ? -1.f : 1.f;
+#pragma unroll
+        for (int k = 0; k < NC; k++) {
+            const uint32_t x[4] = {u[k].x, u[k].y, u[k].z, u[k].w};
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                q[k][e] = (_Float16) ldexpf(sign * (e & 1 ? bf_hi(x[e / 2]) : bf_lo(x[e / 2])), 8 - e2);
+        }
+    }
+    f32x16 o[ND];
+#pragma unroll
+    for (int t = 0; t < ND; t++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) o[t][e] = 0.f;
+    float m = -inf, l = 0.f;
+    int eref = -1000, emax = -1000;                              // no page yet
+
+    float sk, sv, skn, svn;
+    int id = page_id(pbeg), idn = page_id(pbeg + 1);
+    if (pbeg < pend) {
+        load(id);
+        scale_of(id, sk, sv);
+        store(page);
+        if (pbeg + 1 < pend) {
+            load(idn);
+            scale_of(idn, skn, svn);
+        }
+    }
+    for (int pg = pbeg; pg < pend; pg++) {
+        const uint4 * cur = page + ((pg - pbeg) & 1) * FRAGS * 64;
+        __syncthreads();                                         // cur is whole, the other buffer is read
+        const float skc = sk, svc = sv;
+        if (pg + 1 < pend) {
+            store(page + ((pg + 1 - pbeg) & 1) * FRAGS * 64);
+            sk = skn;
+            sv = svn;
+            if (pg + 2 < pend) {
+                const int id2 = page_id(pg + 2);
+                load(id2);
+                scale_of(id2, skn, svn);
+            }
+        }
+        const int t0 = pg * KV8_PAGE;
+        if (!live || t0 >= wlast.hi || t0 + KV8_PAGE <= wfirst.lo) continue;
+        f32x16 sc[2];
+#pragma unroll
+        for (int T = 0; T < 2; T++) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) sc[T][e] = 0.f;
+#pragma unroll
+            for (int k = 0; k < NC; k++)
+                sc[T] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, cur[(T * NC + k) * 64 + lane]), q[k], sc[T], 0, 0, 0);
+        }
+        const float cs0 = rowf * skc, cs = cs0 < 1e-35f ? 1e-35f : cs0;      // (above 0, so that -inf stays -inf; a NaN stays)
+        const bool edge = t0 < wlast.lo || t0 + KV8_PAGE > wfirst.hi || t0 < lo || t0 + KV8_PAGE > hi;
+        if (MASK) {
+            const __amdgpu_buffer_rsrc_t mr = __builtin_amdgcn_make_buffer_rsrc(
+                (void *) (a.mask + i * a.mld + t0), (short) 0, 4 * (hi - t0 < KV8_PAGE ? hi - t0 : KV8_PAGE), 0x00020000);
+#pragma unroll
+            for (int T = 0; T < 2; T++)
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    sc[T][e] = fmaf(sc[T][e], cs, __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+                                                      mr, 4 * (32 * T + 8 * (e >> 2) + 4 * half + (e & 3)), 0, 0)));
+        }
+        if (edge) {
+            const int l0 = (mine.lo > lo ? mine.lo : lo) - t0 - 4 * half, h0 = (mine.hi < hi ? mine.hi : hi) - t0 - 4 * half;
+#pragma unroll
+            for (int T = 0; T < 2; T++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const int n = 32 * T + 8 * (e >> 2) + (e & 3);
+                    sc[T][e] = n >= l0 && n < h0 ? sc[T][e] : -inf;
+                }
+        }
+        float mx = sc[0][0];
+#pragma unroll
+        for (int T = 0; T < 2; T++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) mx = fmaxf(mx, sc[T][e]);
+        {
+            typedef unsigned u2 __attribute__((ext_vector_type(2)));
+            const u2 x = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+            mx = fmaxf(__uint_as_float(x.x), __uint_as_float(x.y));
+        }
+        if (!MASK) mx *= cs;
+        // V's scale as a power of two within 2^4 of the reference, which moves otherwise (never 2^60 below the largest)
+        float ls = __builtin_amdgcn_logf(svc < 1e-36f ? 1e-36f : svc);       // log2; of a NaN NaN
+        const bool poison = !(ls < 128.f);
+        if (poison) ls = eref > -1000 ? (float) eref : 0.f;
+        const float step = MASK ? 3.f / LOG2E : 3.f;
+        const bool move = mx > m + step || (m == -inf && mx > m);
+        const bool shift = fabsf(ls - (float) eref) > 4.f;
+        if (__any(move) || shift) {
+            const float mn = move ? mx : m, base = mn == -inf ? 0.f : mn;
+            float f = m == -inf ? 0.f : __builtin_amdgcn_exp2f(MASK ? (m - base) * LOG2E : m - base);
+            l *= f;
+            m = mn;
+            if (shift) {
+                int e = (int) rintf(ls);
+                emax = e > emax ? e : emax;
+                e = e < emax - 60 ? emax - 60 : e;
+                f = ldexpf(f, eref - e > 200 ? 200 : (eref - e < -200 ? -200 : eref - e));
+                eref = e;
+            }
+#pragma unroll
+            for (int t = 0; t < ND; t++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[t][e] *= f;
+        }
+        // weights: 2^8 e^(x - m) sv 2^-eref in fp16
+        const float base = m == -inf ? 0.f : m, lr = 8.f + (ls - (float) eref);
+        float k = cs, off = lr - base;
+        if (!MASK && __any(fabsf(base) > 65536.f)) {             // there a score's own rounding counts, as m has it
+#pragma unroll
+            for (int T = 0; T < 2; T++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    float x = sc[T][e] * cs;
+                    asm volatile("" : "+v"(x));                  // (not fused with the difference)
+                    sc[T][e] = x - base;
+                }
+            k = 1.f;
+            off = lr;
+        }
+        f16x2 p[2][8];
+        float sum = 0.f;
+        const f16x2 one = {(_Float16) 1.f, (_Float16) 1.f};
+#pragma unroll
+        for (int T = 0; T < 2; T++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                f32x2 y;
+#pragma unroll
+                for (int v = 0; v < 2; v++)
+                    y[v] = __builtin_amdgcn_exp2f(MASK ? fmaf(sc[T][2 * e + v] - base, LOG2E, lr) : fmaf(sc[T][2 * e + v], k, off));
+                p[T][e] = __builtin_convertvector(y, f16x2);
+                sum = __builtin_amdgcn_fdot2(p[T][e], one, sum, false);
+            }
+        l = fmaf(sum, __builtin_amdgcn_exp2f(-lr), l);
+        if (poison && mine.lo < t0 + KV8_PAGE && mine.hi > t0) l = nan;
+#pragma unroll
+        for (int T = 0; T < 2; T++)
+#pragma unroll
+            for (int v = 0; v < 2; v++) {
+                f16x8 b;
+#pragma unroll
+                for (int e = 0; e < 8; e++) b[e] = p[T][2 * (v + 2 * (e >> 2)) + ((e & 3) >> 1)][e & 1];
+#pragma unroll
+                for (int t = 0; t < ND; t++)
+                    o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                        __builtin_bit_cast(f16x8, cur[(2 * NC + t * 4 + T * 2 + v) * 64 + lane]), b, o[t], 0, 0, 0);
+            }
+    }
+    if (!live || w * 32 + n31 >= nrow) return;
+    {
+        typedef unsigned u2 __attribute__((ext_vector_type(2)));
+        const u2 x = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+        l = __uint_as_float(x.x) + __uint_as_float(x.y);
+    }
+    const int64_t at = (r.row + j) * a.Hq + h;
+    float f = ldexpf(1.f, eref <= -1000 ? 0 : eref - 8);
+    if (a.nch == 1) {
+        if (a.sinks) {
+            const float base = m == -inf ? 0.f : m;
+            l += __builtin_amdgcn_exp2f(MASK ? (a.sinks[h] - base) * LOG2E : a.sinks[h] * LOG2E - base);
+        }
+        f = l == 0.f ? 0.f : f / l;
+    } else if (half == 0) {
+        float * wml = a.ws + a.t.T * a.Hq * a.nch * D + (at * a.nch + c) * 2;
+        wml[0] = m;
+        wml[1] = l;
+    }
+#pragma unroll
+    for (int t = 0; t < ND; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int d = 32 * t + 8 * e + 4 * half;
+            if (d >= D) continue;
+            const float4 y = make_float4(o[t][4 * e] * f, o[t][4 * e + 1] * f, o[t][4 * e + 2] * f, o[t][4 * e + 3] * f);
+            if (a.nch > 1) *(float4 *) (a.ws + (at * a.nch + c) * D + d) = y;
+            else *(uint2 *) ((uint16_t *) a.out + at * D + d) =
+                make_uint2(f32_to_bf16(y.x) | (uint32_t) f32_to_bf16(y.y) << 16, f32_to_bf16(y.z) | (uint32_t) f32_to_bf16(y.w) << 16);
+        }
+}
+
 // The chunks of a row joined: a workgroup per (row, head). A wave finds the largest maximum and the
 // weights, a chunk a lane; every thread then adds its column over its share of the chunks.
 __global__ __launch_bounds__(KT) void k_kv8_combine(Kv8AttnArgs a) {
@@ -502,21 +806,25 @@ __global__ __launch_bounds__(KT) void k_kv8_combine(Kv8AttnArgs a) {
     }
 }
 
-struct AttnPlan { int RS, ngrp, C, nch; };
+// tile: k_kv8_tile's plan, else k_kv8_step's
+struct AttnPlan { bool tile; int RS, ngrp, C, nch, fold; };
 
-AttnPlan attn_plan(int Hq, int Hkv, int nseq, int max_n, int max_len, int window) {
+AttnPlan attn_plan(int f32, int Hq, int Hkv, int nseq, int max_n, int max_len, int window) {
     AttnPlan p;
     const int64_t rows = (int64_t) max_n * (Hq / Hkv);
+    p.tile = !f32 && rows > 16;
     p.RS = rows <= 4 ? 1 : (rows <= 8 ? 2 : 4);
-    p.ngrp = (int) ((rows + 4 * p.RS - 1) / (4 * p.RS));
-    // chunks of whole rounds of the waves
-    const int64_t round = SW * KV8_PAGE, wgs = (int64_t) Hkv * p.ngrp * nseq;
-    int64_t nch = (1024 + wgs - 1) / wgs, most = (max_len + round - 1) / round;
+    const int group = p.tile ? TR : 4 * p.RS;
+    p.ngrp = (int) ((rows + group - 1) / group);
+    const int64_t wgs = (int64_t) Hkv * p.ngrp * nseq, round = p.tile ? KV8_PAGE : SW * KV8_PAGE;
+    // step: chunks of whole rounds of the waves; tile: enough workgroups for two a CU, chunks of 512 tokens or more
+    int64_t nch = ((p.tile ? 512 : 1024) + wgs - 1) / wgs, most = (max_len + (p.tile ? 511 : round - 1)) / (p.tile ? 512 : round);
     if (nch > most) nch = most;
     int64_t C = (max_len + nch - 1) / nch;
     C = (C + round - 1) / round * round;
     p.C = (int) (C > (1 << 30) ? 1 << 30 : C);
     p.nch = (int) ((max_len + (int64_t) p.C - 1) / p.C);
+    p.fold = wgs * p.nch <= 512;
     return p;
 }
 
@@ -525,14 +833,16 @@ template <int NC, int RS> hipError_t run_step(const Kv8AttnArgs & a, const AttnP
     const size_t lds = sizeof(float) * SW * 4 * RS * (a.c.D + 2);
     if (a.mask) k_kv8_step<NC, RS, true><<<grid, KT, lds, s>>>(a);
     else k_kv8_step<NC, RS, false><<<grid, KT, lds, s>>>(a);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || p.nch == 1) return e;
-    k_kv8_combine<<<dim3((unsigned) (a.Hq * a.t.max_n), (unsigned) a.t.nseq), KT, 0, s>>>(a);
     return hipGetLastError();
 }
 
-template <int NC> hipError_t run_step_rs(const Kv8AttnArgs & a, const AttnPlan & p, hipStream_t s) {
-    return p.RS == 1 ? run_step<NC, 1>(a, p, s) : (p.RS == 2 ? run_step<NC, 2>(a, p, s) : run_step<NC, 4>(a, p, s));
+template <int NC> hipError_t run_attn(const Kv8AttnArgs & a, const AttnPlan & p, hipStream_t s) {
+    if (!p.tile) return p.RS == 1 ? run_step<NC, 1>(a, p, s) : (p.RS == 2 ? run_step<NC, 2>(a, p, s) : run_step<NC, 4>(a, p, s));
+    const dim3 grid((unsigned) (a.c.Hkv * p.ngrp), (unsigned) p.nch, (unsigned) a.t.nseq);
+    const size_t lds = 2 * 4 * NC * 1024;
+    if (a.mask) k_kv8_tile<NC, true><<<grid, KT, lds, s>>>(a);
+    else k_kv8_tile<NC, false><<<grid, KT, lds, s>>>(a);
+    return hipGetLastError();
 }
 
 }  // namespace
@@ -559,19 +869,22 @@ hipError_t launch_kv8_read(const Kv8Cache & c, const Kv8Table & t, void * k, voi
     return hipGetLastError();
 }
 
-int64_t kv8_attn_ws_bytes(int Hq, int D, int Hkv, int nseq, int64_t T, int max_n, int max_len, int window) {
-    const AttnPlan p = attn_plan(Hq, Hkv, nseq, max_n, max_len, window);
+int64_t kv8_attn_ws_bytes(int f32, int Hq, int D, int Hkv, int nseq, int64_t T, int max_n, int max_len, int window) {
+    const AttnPlan p = attn_plan(f32, Hq, Hkv, nseq, max_n, max_len, window);
     return p.nch == 1 ? 0 : T * Hq * p.nch * (D + 2) * (int64_t) sizeof(float);
 }
 
 hipError_t launch_kv8_attn(const Kv8Cache & c, const Kv8Table & t, const void * q, int f32, int Hq, int64_t qrs, int64_t qhs,
                            int max_len, const float * mask, int64_t mld, const float * sinks, int window, float scale,
                            void * out, void * ws, hipStream_t s) {
-    const AttnPlan p = attn_plan(Hq, c.Hkv, t.nseq, t.max_n, max_len, window);
-    Kv8AttnArgs a{c, t, q, out, mask, sinks, (float *) ws, qrs, qhs, mld, scale, Hq, Hq / c.Hkv, max_len, window, f32, p.C, p.nch};
+    const AttnPlan p = attn_plan(f32, Hq, c.Hkv, t.nseq, t.max_n, max_len, window);
+    Kv8AttnArgs a{c, t, q, out, mask, sinks, (float *) ws, qrs, qhs, mld, scale, Hq, Hq / c.Hkv, max_len, window, f32, p.C, p.nch, p.fold};
     if (!grid_fits((int64_t) Hq * t.max_n, t.nseq) || !grid_fits((int64_t) c.Hkv * p.ngrp, t.nseq) || p.nch > 65535)
         return hipErrorInvalidValue;
     const int nc = c.D / 16;
-    return nc <= 4 ? run_step_rs<4>(a, p, s) : (nc <= 6 ? run_step_rs<6>(a, p, s) : (nc <= 8 ? run_step_rs<8>(a, p, s) :
-           (nc <= 12 ? run_step_rs<12>(a, p, s) : run_step_rs<16>(a, p, s))));
+    hipError_t e = nc <= 4 ? run_attn<4>(a, p, s) : (nc <= 6 ? run_attn<6>(a, p, s) : (nc <= 8 ? run_attn<8>(a, p, s) :
+                   (nc <= 12 ? run_attn<12>(a, p, s) : run_attn<16>(a, p, s))));
+    if (e != hipSuccess || p.nch == 1) return e;
+    k_kv8_combine<<<dim3((unsigned) (Hq * t.max_n), (unsigned) t.nseq), KT, 0, s>>>(a);
+    return hipGetLastError();
 }

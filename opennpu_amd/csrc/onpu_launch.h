@@ -278,7 +278,7 @@ hipError_t launch_attn_step(const float * q, int Hq, int D, const void * K, cons
 hipError_t launch_kv8_write(const Kv8Cache & c, const Kv8Table & t, const void * k, const void * v, int f32, int64_t krs,
                             int64_t khs, int64_t vrs, int64_t vhs, hipStream_t s);
 hipError_t launch_kv8_read(const Kv8Cache & c, const Kv8Table & t, void * k, void * v, int f32, hipStream_t s);
-int64_t kv8_attn_ws_bytes(int Hq, int D, int Hkv, int nseq, int64_t T, int max_n, int max_len, int window);
+int64_t kv8_attn_ws_bytes(int f32, int Hq, int D, int Hkv, int nseq, int64_t T, int max_n, int max_len, int window);
 hipError_t launch_kv8_attn(const Kv8Cache & c, const Kv8Table & t, const void * q, int f32, int Hq, int64_t qrs, int64_t qhs,
                            int max_len, const float * mask, int64_t mld, const float * sinks, int window, float scale,
                            void * out, void * ws, hipStream_t s);

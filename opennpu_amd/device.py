@@ -342,7 +342,7 @@ def kv8_attn(q, codes, scales, table, lens, off=None, max_n=None, max_len=None, 
         if t is not None and (t.dtype != torch.float32 or not t.is_cuda or t.get_device() != q.get_device() or t.stride(-1) != 1
                               or (t.shape != shape if shape else t.dim() != 2 or t.shape[0] != nseq or t.shape[1] < max_len)):
             raise ValueError("kv8_attn: mask must be fp32 [sequences][>= max_len], sinks fp32 [Hq], on q's GPU")
-    nb = L.onpu_kv8_attn_ws_bytes(Hq, D, Hkv, nseq, T, n, max_len, window)
+    nb = L.onpu_kv8_attn_ws_bytes(int(q.dtype == torch.bfloat16), Hq, D, Hkv, nseq, T, n, max_len, window)
     if nb and ws is None:
         ws = torch.empty((nb,), dtype=torch.uint8, device=q.device)
     check(L.onpu_kv8_attn_dev(_ptr(q), int(q.dtype == torch.bfloat16), Hq, q.stride(0), q.stride(1), _ptr(codes),

@@ -133,7 +133,7 @@ def test_refusals(name):
 
 def test_short_workspace_is_refused():
     L = _lib.lib()
-    need = L.onpu_kv8_attn_ws_bytes(4, 64, 2, 2, 5, 4, 100000, 0)
+    need = L.onpu_kv8_attn_ws_bytes(1, 4, 64, 2, 2, 5, 4, 100000, 0)
     if need:
         args = dict(_Args.BASE["attn"], max_len=100000)
         for bad in (dict(ws_bytes=need - 1), dict(ws=None), dict(ws=(1 << 20) + 4)):
