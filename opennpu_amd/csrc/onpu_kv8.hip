@@ -13,25 +13,26 @@ constexpr int KT = 256;                       // threads per workgroup
 __device__ __forceinline__ float bf_lo(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float bf_hi(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
 
-// 16 consecutive values, fp32 or bf16
+// 16 (8) consecutive values, fp32 or bf16, as they lie
+template <bool F32> struct Raw16 { uint4 u[F32 ? 4 : 2]; };
+template <bool F32> struct Raw8 { uint4 u[F32 ? 2 : 1]; };
+template <bool F32, class R> __device__ __forceinline__ R load_raw(const void * base, int64_t at) {
+    const uint4 * p = F32 ? (const uint4 *) ((const float *) base + at) : (const uint4 *) ((const uint16_t *) base + at);
+    R r;
+#pragma unroll
+    for (size_t i = 0; i < sizeof(R) / 16; i++) r.u[i] = p[i];
+    return r;
+}
+template <bool F32, class R> __device__ __forceinline__ float raw_at(const R & r, int e) {
+    const uint4 u = r.u[F32 ? e >> 2 : e >> 3];
+    const int w = F32 ? e & 3 : (e >> 1) & 3;
+    const uint32_t x = w == 0 ? u.x : (w == 1 ? u.y : (w == 2 ? u.z : u.w));
+    return F32 ? __uint_as_float(x) : (e & 1 ? bf_hi(x) : bf_lo(x));
+}
 template <bool F32> __device__ __forceinline__ void load16(const void * base, int64_t at, float (&x)[16]) {
-    if (F32) {
-        const uint4 * p = (const uint4 *) ((const float *) base + at);
+    const Raw16<F32> r = load_raw<F32, Raw16<F32>>(base, at);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint4 u = p[i];
-            x[4 * i] = __uint_as_float(u.x); x[4 * i + 1] = __uint_as_float(u.y);
-            x[4 * i + 2] = __uint_as_float(u.z); x[4 * i + 3] = __uint_as_float(u.w);
-        }
-    } else {
-        const uint4 * p = (const uint4 *) ((const uint16_t *) base + at);
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const uint4 u = p[i];
-            x[8 * i] = bf_lo(u.x); x[8 * i + 1] = bf_hi(u.x); x[8 * i + 2] = bf_lo(u.y); x[8 * i + 3] = bf_hi(u.y);
-            x[8 * i + 4] = bf_lo(u.z); x[8 * i + 5] = bf_hi(u.z); x[8 * i + 6] = bf_lo(u.w); x[8 * i + 7] = bf_hi(u.w);
-        }
-    }
+    for (int e = 0; e < 16; e++) x[e] = raw_at<F32>(r, e);
 }
 
 // ------------------------------------------------------------------ write
@@ -40,7 +41,10 @@ template <bool F32> __device__ __forceinline__ void load16(const void * base, in
 // rescaled when s grew), code = x / s to the nearest, ties to even, of the exact quotient: with c the
 // nearest integer of x * (1 / s), x - c s is exact in one fma (a multiple of half an ulp of s and below s), so that
 // a c one off near a border is put right by comparing it with s / 2. A value that is not finite makes
-// the page's scale NaN, and all that is read of it.
+// the page's scale NaN, and all that is read of it. Bound by the bytes for prompts: each value is read once
+// and stays in registers across the maximum (a lane has 16 d of a K token and 8 d of 4 V tokens, so that
+// V's bytes of 4 tokens are whole words); K's codes go out from there, V's through LDS in the page's
+// order. A page with earlier tokens is changed in place, its new bytes alone unless the scale grows.
 struct WriteArgs {
     Kv8Cache c;
     Kv8Table t;
@@ -57,10 +61,20 @@ __device__ __forceinline__ int quant(float x, float s, float inv) {
     if (e < -h || (e == -h && odd)) c -= 1.f;
     return (int) fminf(fmaxf(c, -127.f), 127.f);
 }
+__device__ __forceinline__ uint32_t bytes4(int a, int b, int c, int d) {
+    return (uint32_t) (a & 255) | (uint32_t) (b & 255) << 8 | (uint32_t) (c & 255) << 16 | (uint32_t) d << 24;
+}
 
-template <bool F32>
+// the scale of values whose largest magnitude has these bits
+__device__ __forceinline__ float scale_for(uint32_t bits) {
+    return bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(__uint_as_float(bits), KV8_TINY) / 127.f;
+}
+
+// NQ: D up to 128 NQ
+template <bool F32, int NQ>
 __global__ __launch_bounds__(KT) void k_kv8_write(WriteArgs a) {
-    extern __shared__ __align__(16) int8_t tile[];               // K's 64 D codes, then V's
+    constexpr int NK = 2 * NQ, NV = NQ;       // units of a lane: 16 d of one K token, 8 d of 4 V tokens
+    extern __shared__ __align__(16) uint32_t vt[];               // V's 64 D codes
     __shared__ uint32_t wmax[2][KT / 64];
     const int D = a.c.D, NC = D / 16, t = threadIdx.x, g = blockIdx.x % a.c.Hkv, w = blockIdx.x / a.c.Hkv, i = blockIdx.y;
     const Kv8Rows r = kv8_rows(a.t.off, i, a.t.T, a.t.max_n);
@@ -69,57 +83,151 @@ __global__ __launch_bounds__(KT) void k_kv8_write(WriteArgs a) {
     const int id = kv8_page(a.t.table + i * a.t.tld, pg, a.t.P, a.c.pages);
     if (id < 0) return;
     const int s0 = p0 > base ? (int) (p0 - base) : 0, s1 = p0 + r.n - base < KV8_PAGE ? (int) (p0 + r.n - base) : KV8_PAGE;
-    const int64_t row0 = r.row + (base + s0 - p0);               // the row of slot s0
-    const int units = (s1 - s0) * NC;
+    const int64_t row0 = r.row + (base - p0);                    // the row of slot 0 (below the sequence's for s0 > 0)
     int8_t * out = a.c.codes + ((int64_t) id * a.c.Hkv + g) * 2 * KV8_PAGE * D;
     float * sc = a.c.scales + ((int64_t) id * a.c.Hkv + g) * 2;
-    float x[16];
+    const float so[2] = {s0 > 0 ? sc[0] : 0.f, s0 > 0 ? sc[1] : 0.f};
+    const bool some = s1 - s0 < 8;            // few tokens: a lane has one value at a time
     uint32_t m[2] = {0, 0};
-    for (int u = t; u < units; u += KT)
-        for (int kv = 0; kv < 2; kv++) {
-            load16<F32>(a.x[kv], (row0 + u / NC) * a.rs[kv] + g * a.hs[kv] + u % NC * 16, x);
-            for (int e = 0; e < 16; e++) m[kv] = max(m[kv], __float_as_uint(x[e]) & 0x7fffffffu);    // NaN the largest
+    Raw16<F32> xk[NK];
+    Raw8<F32> xv[NV][4];
+    if (some) {
+        for (int kv = 0; kv < 2; kv++)
+            for (int u = t; u < (s1 - s0) * D; u += KT) {
+                const int64_t at = (row0 + s0 + u / D) * a.rs[kv] + g * a.hs[kv] + u % D;
+                m[kv] = max(m[kv], (F32 ? ((const uint32_t *) a.x[kv])[at] : (uint32_t) ((const uint16_t *) a.x[kv])[at] << 16) & 0x7fffffffu);
+            }
+    } else {
+#pragma unroll
+        for (int k = 0; k < NK; k++) {
+            const int u = t + KT * k, tok = u / NC, ok = tok >= s0 && tok < s1;
+            xk[k] = load_raw<F32, Raw16<F32>>(a.x[0], (row0 + (ok ? tok : s0)) * a.rs[0] + g * a.hs[0] + u % NC * 16);
         }
+#pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const int u = t + KT * k, q = u / (2 * NC), d = u % (2 * NC) * 8;      // tokens 4 q .. 4 q + 3
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int tok = 4 * q + e, ok = tok >= s0 && tok < s1;
+                xv[k][e] = load_raw<F32, Raw8<F32>>(a.x[1], (row0 + (ok ? tok : s0)) * a.rs[1] + g * a.hs[1] + d);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < NK; k++)          // (slots outside repeat slot s0: the maximum is of the new values)
+#pragma unroll
+            for (int e = 0; e < 16; e++) m[0] = max(m[0], __float_as_uint(raw_at<F32>(xk[k], e)) & 0x7fffffffu);
+#pragma unroll
+        for (int k = 0; k < NV; k++)
+#pragma unroll
+            for (int e = 0; e < 32; e++) m[1] = max(m[1], __float_as_uint(raw_at<F32>(xv[k][e >> 3], e & 7)) & 0x7fffffffu);
+    }
+#pragma unroll
     for (int kv = 0; kv < 2; kv++) {
-        for (int o = 32; o > 0; o >>= 1) m[kv] = max(m[kv], (uint32_t) __shfl_xor((int) m[kv], o));
+        for (int o = 32; o > 0; o >>= 1) m[kv] = max(m[kv], (uint32_t) __shfl_xor((int) m[kv], o));       // (NaN is the largest)
         if ((t & 63) == 0) wmax[kv][t >> 6] = m[kv];
     }
-    float s[2], so[2];
-    for (int kv = 0; kv < 2; kv++) so[kv] = s0 > 0 ? sc[kv] : 0.f;
-    // the page as it is (zeros for a new one)
-    uint4 * tl = (uint4 *) tile;
-    for (int u = t; u < 8 * D; u += KT) tl[u] = s0 > 0 ? ((const uint4 *) out)[u] : make_uint4(0, 0, 0, 0);
     __syncthreads();
+    float s[2], inv[2];
+#pragma unroll
     for (int kv = 0; kv < 2; kv++) {
         uint32_t b = wmax[kv][0];
+#pragma unroll
         for (int k = 1; k < KT / 64; k++) b = max(b, wmax[kv][k]);
-        s[kv] = b >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(__uint_as_float(b), KV8_TINY) / 127.f;
+        s[kv] = scale_for(b);
         if (s0 > 0 && !(so[kv] <= s[kv])) s[kv] = s[kv] != s[kv] ? s[kv] : so[kv];          // (a NaN stays)
-        if (s0 > 0 && s[kv] > so[kv]) {
+        inv[kv] = 1.f / s[kv];
+        if (s0 > 0 && s[kv] > so[kv]) {       // the earlier codes in the new scale
             const double f = (double) so[kv] / (double) s[kv];
-            for (int u = t; u < KV8_PAGE * D; u += KT) {
-                int8_t * p = tile + kv * KV8_PAGE * D + u;
-                *p = (int8_t) rint(*p * f);
+            uint4 * p = (uint4 *) (out + kv * KV8_PAGE * D);
+            for (int u = t; u < 4 * D; u += KT) {
+                uint32_t y[4] = {p[u].x, p[u].y, p[u].z, p[u].w};
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    y[e] = bytes4((int) rint((int8_t) y[e] * f), (int) rint((int8_t) (y[e] >> 8) * f),
+                                  (int) rint((int8_t) (y[e] >> 16) * f), (int) rint((int8_t) (y[e] >> 24) * f));
+                p[u] = make_uint4(y[0], y[1], y[2], y[3]);
             }
         }
     }
-    __syncthreads();
-    for (int u = t; u < units; u += KT)
-        for (int kv = 0; kv < 2; kv++) {
-            load16<F32>(a.x[kv], (row0 + u / NC) * a.rs[kv] + g * a.hs[kv] + u % NC * 16, x);
-            const float inv = 1.f / s[kv];
-            const int token = s0 + u / NC, d = u % NC * 16;
-            for (int e = 0; e < 16; e++)
-                tile[kv ? KV8_PAGE * D + kv8_v_at(D, token, d + e) : kv8_k_at(D, token, d + e)] = (int8_t) quant(x[e], s[kv], inv);
+    if (s0 > 0) __syncthreads();              // the new bytes go on top (and so has been read by all)
+    if (t < 2) sc[t] = t ? s[1] : s[0];
+    if (some && s0 > 0) {
+        for (int kv = 0; kv < 2; kv++)
+            for (int u = t; u < (s1 - s0) * D; u += KT) {
+                const int tok = s0 + u / D, d = u % D;
+                const int64_t at = (row0 + tok) * a.rs[kv] + g * a.hs[kv] + d;
+                const float x = F32 ? ((const float *) a.x[kv])[at] : bf16_to_f32(((const uint16_t *) a.x[kv])[at]);
+                out[kv ? KV8_PAGE * D + kv8_v_at(D, tok, d) : kv8_k_at(D, tok, d)] = (int8_t) quant(x, s[kv], inv[kv]);
+            }
+        return;
+    }
+    if (some) {                               // a page begun by a few tokens
+        for (int u = t; u < 16 * D; u += KT) {
+            const int tok = u / (D / 4), d = u % (D / 4) * 4;
+            uint32_t y = 0;
+            if (tok < s1) {
+                int q[4];
+                for (int e = 0; e < 4; e++) {
+                    const int64_t at = (row0 + tok) * a.rs[0] + g * a.hs[0] + d + e;
+                    q[e] = quant(F32 ? ((const float *) a.x[0])[at] : bf16_to_f32(((const uint16_t *) a.x[0])[at]), s[0], inv[0]);
+                }
+                y = bytes4(q[0], q[1], q[2], q[3]);
+            }
+            *(uint32_t *) (out + kv8_k_at(D, tok, d)) = y;
+            const int vq = u / D, vd = u % D;                    // tokens 4 vq .. 4 vq + 3
+            y = 0;
+            for (int e = 0; e < 4; e++)
+                if (4 * vq + e < s1) {
+                    const int64_t at = (row0 + 4 * vq + e) * a.rs[1] + g * a.hs[1] + vd;
+                    y |= (uint32_t) (quant(F32 ? ((const float *) a.x[1])[at] : bf16_to_f32(((const uint16_t *) a.x[1])[at]), s[1], inv[1]) & 255) << (8 * e);
+                }
+            *(uint32_t *) (out + KV8_PAGE * D + kv8_v_at(D, 4 * vq, vd)) = y;
         }
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < NK; k++) {
+        const int u = t + KT * k, tok = u / NC, d = u % NC * 16;
+        if (tok >= KV8_PAGE || tok < s0 || (s0 > 0 && tok >= s1)) continue;
+        uint32_t y[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            y[e] = bytes4(quant(raw_at<F32>(xk[k], 4 * e), s[0], inv[0]), quant(raw_at<F32>(xk[k], 4 * e + 1), s[0], inv[0]),
+                          quant(raw_at<F32>(xk[k], 4 * e + 2), s[0], inv[0]), quant(raw_at<F32>(xk[k], 4 * e + 3), s[0], inv[0]));
+            if (tok >= s1) y[e] = 0;
+        }
+        *(uint4 *) (out + kv8_k_at(D, tok, d)) = make_uint4(y[0], y[1], y[2], y[3]);
+    }
+    const bool merge = s0 > 0;                // V's words of the page as they are below the new bytes
+    int8_t * ov = out + KV8_PAGE * D;
+#pragma unroll
+    for (int k = 0; k < NV; k++) {
+        const int u = t + KT * k, q = u / (2 * NC), d = u % (2 * NC) * 8;
+        if (q >= 16) continue;
+        uint32_t keep = 0;                    // bytes of tokens that are not new
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (4 * q + e < s0 || 4 * q + e >= s1) keep |= 255u << (8 * e);
+        if (merge && keep == 0xffffffffu) continue;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int at = kv8_v_at(D, 4 * q, d + e);
+            const uint32_t y = bytes4(quant(raw_at<F32>(xv[k][0], e), s[1], inv[1]), quant(raw_at<F32>(xv[k][1], e), s[1], inv[1]),
+                                      quant(raw_at<F32>(xv[k][2], e), s[1], inv[1]), quant(raw_at<F32>(xv[k][3], e), s[1], inv[1]));
+            if (merge) *(uint32_t *) (ov + at) = (y & ~keep) | (keep ? *(uint32_t *) (ov + at) & keep : 0);
+            else vt[at / 4] = y & ~keep;
+        }
+    }
+    if (merge) return;
     __syncthreads();
-    for (int u = t; u < 8 * D; u += KT) ((uint4 *) out)[u] = tl[u];
-    if (t < 2) sc[t] = s[t];
+    for (int u = t; u < 4 * D; u += KT) ((uint4 *) ov)[u] = ((const uint4 *) vt)[u];
 }
 
 // ------------------------------------------------------------------ read
-// A workgroup per (page, kv head, sequence): value = code * scale, one rounding (two for bf16: to fp32
-// and then to bf16). A page that the table does not have reads as NaN.
+// A workgroup per (page, kv head, sequence): value = code * scale, rounded once (bf16: that rounded
+// again); code + 128 by an unsigned byte's conversion, less 128 in the product's fma, whose one rounding is
+// the product's. A page that the table does not have reads as NaN. Bound by the bytes: a lane writes 16 d
+// of a K token and 8 d of 4 V tokens, V's words turned through LDS.
 struct ReadArgs {
     Kv8Cache c;
     Kv8Table t;
@@ -127,27 +235,62 @@ struct ReadArgs {
     int W;
 };
 
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+}
+
+// N values (8 or 16) to row `at` of y
+template <bool F32, int N> __device__ __forceinline__ void put(void * y, int64_t at, const float (&v)[N]) {
+    if (F32) {
+#pragma unroll
+        for (int e = 0; e < N; e += 4) *(float4 *) ((float *) y + at + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; e += 8)
+            *(uint4 *) ((uint16_t *) y + at + e) = make_uint4(pack_bf16(v[e], v[e + 1]), pack_bf16(v[e + 2], v[e + 3]),
+                                                              pack_bf16(v[e + 4], v[e + 5]), pack_bf16(v[e + 6], v[e + 7]));
+    }
+}
+
 template <bool F32>
 __global__ __launch_bounds__(KT) void k_kv8_read(ReadArgs a) {
+    extern __shared__ __align__(16) uint32_t vt[];               // V's 64 D codes
     const int D = a.c.D, NC = D / 16, t = threadIdx.x, g = blockIdx.x % a.c.Hkv, w = blockIdx.x / a.c.Hkv, i = blockIdx.y;
     const Kv8Rows r = kv8_rows(a.t.off, i, a.t.T, a.t.max_n);
     const int64_t p0 = a.t.pos[i], pg = (p0 - (p0 & (KV8_PAGE - 1))) / KV8_PAGE + w, base = pg * KV8_PAGE;
     if (base >= p0 + r.n) return;
     const int id = kv8_page(a.t.table + i * a.t.tld, pg, a.t.P, a.c.pages);
     const int s0 = p0 > base ? (int) (p0 - base) : 0, s1 = p0 + r.n - base < KV8_PAGE ? (int) (p0 + r.n - base) : KV8_PAGE;
-    const int64_t row0 = r.row + (base + s0 - p0);
+    const int64_t row0 = r.row + (base - p0);
     const int8_t * in = a.c.codes + ((int64_t) (id < 0 ? 0 : id) * a.c.Hkv + g) * 2 * KV8_PAGE * D;
     const float * sc = a.c.scales + ((int64_t) (id < 0 ? 0 : id) * a.c.Hkv + g) * 2;
-    for (int kv = 0; kv < 2; kv++) {
-        const float s = id < 0 ? __uint_as_float(0x7fc00000u) : sc[kv];
-        for (int u = t; u < (s1 - s0) * NC; u += KT) {
-            const int token = s0 + u / NC, d = u % NC * 16;
-            const int64_t at = ((row0 + u / NC) * a.c.Hkv + g) * D + d;
-            for (int e = 0; e < 16; e++) {
-                const float v = in[kv ? KV8_PAGE * D + kv8_v_at(D, token, d + e) : kv8_k_at(D, token, d + e)] * s;
-                if (F32) ((float *) a.y[kv])[at + e] = v;
-                else ((uint16_t *) a.y[kv])[at + e] = f32_to_bf16(v);
-            }
+    for (int u = t; u < 4 * D; u += KT) ((uint4 *) vt)[u] = ((const uint4 *) (in + KV8_PAGE * D))[u];
+    const float nan = __uint_as_float(0x7fc00000u), sk = id < 0 ? nan : sc[0], sv = id < 0 ? nan : sc[1];
+    for (int u = s0 * NC + t; u < s1 * NC; u += KT) {
+        const int tok = u / NC, d = u % NC * 16;
+        const uint4 c = *(const uint4 *) (in + kv8_k_at(D, tok, d));
+        const uint32_t x[4] = {c.x ^ 0x80808080u, c.y ^ 0x80808080u, c.z ^ 0x80808080u, c.w ^ 0x80808080u};
+        float v[16];
+#pragma unroll
+        for (int e = 0; e < 16; e++) v[e] = fmaf((float) (x[e >> 2] >> (8 * (e & 3)) & 255), sk, -128.f * sk);
+        put<F32, 16>(a.y[0], ((row0 + tok) * a.c.Hkv + g) * D + d, v);
+    }
+    __syncthreads();
+    for (int u = (s0 >> 2) * 2 * NC + t; u < ((s1 + 3) >> 2) * 2 * NC; u += KT) {
+        const int q = u / (2 * NC), d = u % (2 * NC) * 8;
+        uint32_t x[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = vt[kv8_v_at(D, 4 * q, d + e) / 4] ^ 0x80808080u;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            if (4 * q + k < s0 || 4 * q + k >= s1) continue;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = fmaf((float) (x[e] >> (8 * k) & 255), sv, -128.f * sv);
+            put<F32, 8>(a.y[1], ((row0 + 4 * q + k) * a.c.Hkv + g) * D + d, v);
         }
     }
 }
@@ -470,7 +613,6 @@ __global__ __launch_bounds__(KT) void k_kv8_step(Kv8AttnArgs a) {
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 // four codes -> fp16, exactly: 1024 + (code + 128) by its bits, less 1152
 __device__ __forceinline__ void codes_f16(uint32_t u, uint32_t & lo, uint32_t & hi) {
@@ -761,17 +903,23 @@ __global__ __launch_bounds__(KT, NC <= 8 ? 2 : 1) void k_kv8_tile(Kv8AttnArgs a)
         }
 }
 
-// The chunks of a row joined: a workgroup per (row, head). A wave finds the largest maximum and the
-// weights, a chunk a lane; every thread then adds its column over its share of the chunks.
+// The chunks of a row joined: W waves per (row, head), W | 4. A wave finds the largest maximum and the weights,
+// a chunk a lane; then D / 4 lanes (rounded up to 16, 32 or 64) add 4 columns each over every (64 / lanes W)th
+// chunk, 8 loads in flight. Bound by latency for few rows of many chunks, by the bytes of the partials for many
+// rows of few.
+template <int W>
 __global__ __launch_bounds__(KT) void k_kv8_combine(Kv8AttnArgs a) {
-    __shared__ float sred[KT], sw[SW][64], sden[SW];
-    const int D = a.c.D, h = blockIdx.x % a.Hq, j = blockIdx.x / a.Hq, i = blockIdx.y, t = threadIdx.x, lane = t & 63, w = t >> 6;
+    __shared__ float sw[SW][64];
+    __shared__ f32x4 sred[SW][64];
+    const int D = a.c.D, i = blockIdx.y, lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int rh = blockIdx.x * (SW / W) + w / W, h = rh % a.Hq, j = rh / a.Hq, part = w % W;
     const Kv8Rows r = kv8_rows(a.t.off, i, a.t.T, a.t.max_n);
-    if (j >= r.n) return;
+    const bool live = j < r.n;
+    if (W == 1 ? !live : (blockIdx.x * (SW / W)) / a.Hq >= r.n) return;       // (W > 1 meets at a barrier: leave together)
     const int full = a.t.pos[i] < 0 ? 0 : a.t.pos[i], len = full < a.max_len ? full : a.max_len;
     const Kv8Seen s = kv8_seen((int64_t) full - r.n + j, len, a.window);
-    const int ca = s.lo / a.C, cb = s.hi > s.lo ? (s.hi - 1) / a.C + 1 : ca;   // the chunks that this row sees
-    const int64_t o = (r.row + j) * a.Hq + h;
+    const int ca = s.lo / a.C, cb = live && s.hi > s.lo ? (s.hi - 1) / a.C + 1 : ca;         // the chunks that this row sees
+    const int64_t o = (r.row + (live ? j : 0)) * a.Hq + h;
     const float * wo = a.ws + o * a.nch * D, * wml = a.ws + a.t.T * a.Hq * a.nch * D + o * a.nch * 2;
     // (maxima are in powers of 2 without a mask, in powers of e with one: its lowest value has to fit)
     const float unit = a.mask ? LOG2E : 1.f, sink = a.sinks ? a.sinks[h] * (a.mask ? 1.f : LOG2E) : -__builtin_inff();
@@ -779,30 +927,36 @@ __global__ __launch_bounds__(KT) void k_kv8_combine(Kv8AttnArgs a) {
     for (int c = ca + lane; c < cb; c += 64) M = fmaxf(M, wml[2 * c]);
     M = wave_max(M);
     const float base = M == -__builtin_inff() ? 0.f : M;
-    float den = 0.f, y = 0.f;
-    const int DP = D <= 64 ? 64 : (D <= 128 ? 128 : 256), G = KT / DP, d = t % DP, gr = t / DP;
+    const int DL = D <= 64 ? 16 : (D <= 128 ? 32 : 64), G = 64 / DL * W, d = lane % DL * 4, gr = part * (64 / DL) + lane / DL;
+    float den = 0.f;
+    f32x4 y = {0, 0, 0, 0};
     for (int b = ca; b < cb; b += 64) {
-        const int c = b + lane;
-        const float f = c < cb ? __builtin_amdgcn_exp2f((wml[2 * c] - base) * unit) : 0.f;
-        if (c < cb) {
-            const float lc = wml[2 * c + 1];
-            den = lc != lc ? lc : fmaf(f, lc, den);
-        }
+        const int n = cb - b < 64 ? cb - b : 64, c = b + (lane < n ? lane : n - 1);
+        const float f = __builtin_amdgcn_exp2f((wml[2 * c] - base) * unit), lc = wml[2 * c + 1];
+        if (lane < n) den = lc != lc ? lc : fmaf(f, lc, den);
         sw[w][lane] = f;
         __builtin_amdgcn_wave_barrier();
-        const int n = cb - b < 64 ? cb - b : 64;
-        if (d < D)
-            for (int k = gr; k < n; k += G) y = fmaf(sw[w][k], wo[(int64_t) (b + k) * D + d], y);
+        for (int k = gr; k < n; k += 8 * G) {
+            f32x4 x[8];
+            const float * p = wo + (int64_t) b * D + (d < D ? d : 0);
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = *(const f32x4 *) (p + (int64_t) (k + G * e < n ? k + G * e : k) * D);
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (k + G * e < n) y += sw[w][k + G * e] * x[e];
+        }
         __builtin_amdgcn_wave_barrier();
     }
     den = wave_sum(den) + (a.sinks ? __builtin_amdgcn_exp2f((sink - base) * unit) : 0.f);
-    sred[t] = y;
-    __syncthreads();
-    if (t < D && gr == 0) {
-        for (int k = 1; k < G; k++) y += sred[k * DP + t];
-        y = den == 0.f ? 0.f : y / den;
-        if (a.f32) ((float *) a.out)[o * D + t] = y;
-        else ((uint16_t *) a.out)[o * D + t] = f32_to_bf16(y);
+    sred[w][lane] = y;
+    if (W > 1) __syncthreads();
+    else __builtin_amdgcn_wave_barrier();
+    if (live && part == 0 && lane < DL && d < D) {
+        for (int k = 1; k < G; k++) y += sred[w + k / (64 / DL)][(k % (64 / DL)) * DL + lane];
+        const float f = den == 0.f ? 0.f : 1.f / den;
+        const float4 v = make_float4(den == 0.f ? 0.f : y[0] * f, den == 0.f ? 0.f : y[1] * f, den == 0.f ? 0.f : y[2] * f, den == 0.f ? 0.f : y[3] * f);
+        if (a.f32) *(float4 *) ((float *) a.out + o * D + d) = v;
+        else *(uint2 *) ((uint16_t *) a.out + o * D + d) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
     }
 }
 
@@ -855,8 +1009,11 @@ hipError_t launch_kv8_write(const Kv8Cache & c, const Kv8Table & t, const void *
     WriteArgs a{c, t, {k, v}, {krs, vrs}, {khs, vhs}, (int) (((int64_t) t.max_n + KV8_PAGE - 2) / KV8_PAGE + 1)};
     if (!grid_fits((int64_t) a.W * c.Hkv, t.nseq)) return hipErrorInvalidValue;
     const dim3 grid((unsigned) (a.W * c.Hkv), (unsigned) t.nseq);
-    if (f32) k_kv8_write<true><<<grid, KT, 2 * KV8_PAGE * c.D, s>>>(a);
-    else k_kv8_write<false><<<grid, KT, 2 * KV8_PAGE * c.D, s>>>(a);
+    const size_t lds = KV8_PAGE * c.D;
+    if (f32 && c.D <= 128) k_kv8_write<true, 1><<<grid, KT, lds, s>>>(a);
+    else if (f32) k_kv8_write<true, 2><<<grid, KT, lds, s>>>(a);
+    else if (c.D <= 128) k_kv8_write<false, 1><<<grid, KT, lds, s>>>(a);
+    else k_kv8_write<false, 2><<<grid, KT, lds, s>>>(a);
     return hipGetLastError();
 }
 
@@ -864,8 +1021,8 @@ hipError_t launch_kv8_read(const Kv8Cache & c, const Kv8Table & t, void * k, voi
     ReadArgs a{c, t, {k, v}, (int) (((int64_t) t.max_n + KV8_PAGE - 2) / KV8_PAGE + 1)};
     if (!grid_fits((int64_t) a.W * c.Hkv, t.nseq)) return hipErrorInvalidValue;
     const dim3 grid((unsigned) (a.W * c.Hkv), (unsigned) t.nseq);
-    if (f32) k_kv8_read<true><<<grid, KT, 0, s>>>(a);
-    else k_kv8_read<false><<<grid, KT, 0, s>>>(a);
+    if (f32) k_kv8_read<true><<<grid, KT, KV8_PAGE * c.D, s>>>(a);
+    else k_kv8_read<false><<<grid, KT, KV8_PAGE * c.D, s>>>(a);
     return hipGetLastError();
 }
 
@@ -885,6 +1042,8 @@ hipError_t launch_kv8_attn(const Kv8Cache & c, const Kv8Table & t, const void * 
     hipError_t e = nc <= 4 ? run_attn<4>(a, p, s) : (nc <= 6 ? run_attn<6>(a, p, s) : (nc <= 8 ? run_attn<8>(a, p, s) :
                    (nc <= 12 ? run_attn<12>(a, p, s) : run_attn<16>(a, p, s))));
     if (e != hipSuccess || p.nch == 1) return e;
-    k_kv8_combine<<<dim3((unsigned) (Hq * t.max_n), (unsigned) t.nseq), KT, 0, s>>>(a);
+    const int64_t rh = (int64_t) Hq * t.max_n;
+    if (p.nch > 16) k_kv8_combine<4><<<dim3((unsigned) rh, (unsigned) t.nseq), KT, 0, s>>>(a);
+    else k_kv8_combine<1><<<dim3((unsigned) ((rh + SW - 1) / SW), (unsigned) t.nseq), KT, 0, s>>>(a);
     return hipGetLastError();
 }
