@@ -1,6 +1,7 @@
 // The 8-bit key-value cache: quantising tokens into its pages, reading them back, and attention over
 // them. Layout and index arithmetic: onpu_kv8.h.
 #include <algorithm>
+#include <cstdlib>
 
 #include "onpu_launch.h"
 
@@ -622,10 +623,18 @@ __device__ __forceinline__ void codes_f16(uint32_t u, uint32_t & lo, uint32_t & 
     hi = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + k);
 }
 
-constexpr int TR = 32 * SW;                   // rows of a workgroup
-template <int NC, bool MASK>
-__global__ __launch_bounds__(KT, NC <= 8 ? 2 : 1) void k_kv8_tile(Kv8AttnArgs a) {
-    constexpr int NU = NC / 2, ND = NC / 2, FRAGS = 4 * NC;      // load units of a wave, d tiles of 32, KiB of a page
+// a workgroup barrier that orders LDS accesses only: global loads stay in flight across it
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+template <int NC, int WV, bool MASK>
+__global__ __launch_bounds__(64 * WV, NC <= 8 ? 8 / WV : 1) void k_kv8_tile(Kv8AttnArgs a) {
+    constexpr int NU = 2 * NC / WV, ND = NC / 2, FRAGS = 4 * NC, TR = 32 * WV;       // load units of a wave, d tiles of 32, KiB of a
+                                                                                     // page, rows of a workgroup
+    static_assert(NU * WV == 2 * NC, "the waves share a page's units evenly");
     extern __shared__ __align__(16) uint4 page[];                // [2][FRAGS][64]
     const int D = a.c.D, nc = D / 16, lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = blockIdx.y, i = blockIdx.z, half = lane >> 5, n31 = lane & 31;
@@ -636,7 +645,9 @@ __global__ __launch_bounds__(KT, NC <= 8 ? 2 : 1) void k_kv8_tile(Kv8AttnArgs a)
     if (z >= ngrp) return;
     // the longest first; with no more workgroups than run at once, the second half the shortest first, so that
     // what two workgroups of a CU have adds to the same
-    z = a.fold && z >= ngrp / 2 ? z - ngrp / 2 : ngrp - 1 - z;
+    if (a.fold == 1) z = z >= ngrp / 2 ? z - ngrp / 2 : ngrp - 1 - z;
+    else if (a.fold == 2) z = z & 1 ? z / 2 : ngrp - 1 - z / 2;
+    else if (a.fold == 0) z = ngrp - 1 - z;
     const int R0 = z * TR, nrow = rows - R0 < TR ? rows - R0 : TR;
     const int full = a.t.pos[i] < 0 ? 0 : a.t.pos[i], len = full < a.max_len ? full : a.max_len;
     const int64_t at0 = (int64_t) full - r.n;
@@ -652,7 +663,7 @@ __global__ __launch_bounds__(KT, NC <= 8 ? 2 : 1) void k_kv8_tile(Kv8AttnArgs a)
     int src[NU], dst[NU][2];
 #pragma unroll
     for (int u = 0; u < NU; u++) {
-        const int k = w + SW * u;
+        const int k = w + WV * u;
         if (k < NC) {                                            // K: tokens 32 T + n31, chunk 2 s + half
             const int T = k / (NC / 2), s2 = k % (NC / 2), ch = 2 * s2 + half < nc ? 2 * s2 + half : nc - 1;
             src[u] = ((2 * T + (n31 >> 4)) * nc + ch) * 256 + (lane & 15) * 16;
@@ -667,7 +678,7 @@ __global__ __launch_bounds__(KT, NC <= 8 ? 2 : 1) void k_kv8_tile(Kv8AttnArgs a)
     }
     uint4 raw[NU];
     auto load = [&](int id) {
-        const int8_t * p = a.c.codes + ((int64_t) (id < 0 ? 0 : id) * a.c.Hkv + g) * 2 * KV8_PAGE * D;
+        const int8_t * p = a.c.codes + ((int64_t) id * a.c.Hkv + g) * 2 * KV8_PAGE * D;
 #pragma unroll
         for (int u = 0; u < NU; u++) raw[u] = *(const uint4 *) (p + src[u]);
     };
@@ -683,13 +694,18 @@ __global__ __launch_bounds__(KT, NC <= 8 ? 2 : 1) void k_kv8_tile(Kv8AttnArgs a)
             to[dst[u][1]] = y;
         }
     };
-    auto page_id = [&](int p) { return p < pend ? kv8_page(tab, p, a.t.P, a.c.pages) : 0; };
-    auto scale_of = [&](int id, float & k, float & v) {
+    // ids and scales of 64 pages at a time, a page a lane: no load to wait for in the loop
+    int lid = 0;
+    float lsk = 0.f, lls = 0.f;               // K's scale, log2 of V's
+    auto fetch = [&](int p0) {
+        const int id = p0 + lane < pend ? kv8_page(tab, p0 + lane, a.t.P, a.c.pages) : -1;
         const float * p = a.c.scales + ((int64_t) (id < 0 ? 0 : id) * a.c.Hkv + g) * 2;
         const bool bad = id < 0 || full > a.max_len;
-        k = bad ? nan : p[0];
-        v = bad ? nan : p[1];
+        lid = id < 0 ? 0 : id;
+        lsk = bad ? nan : p[0];
+        lls = bad ? nan : __builtin_amdgcn_logf(p[1] < 1e-36f ? 1e-36f : p[1]);
     };
+    auto lane_f = [&](float v, int n) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), n)); };
 
     // this lane's row
     const int rr = w * 32 + n31 < nrow ? w * 32 + n31 : nrow - 1, j = (R0 + rr) / a.rep, h = g * a.rep + (R0 + rr - j * a.rep);
@@ -734,42 +750,55 @@ __global__ __launch_bounds__(KT, NC <= 8 ? 2 : 1) void k_kv8_tile(Kv8AttnArgs a)
     float m = -inf, l = 0.f;
     int eref = -1000, emax = -1000;                              // no page yet
 
-    float sk, sv, skn, svn;
-    int id = page_id(pbeg), idn = page_id(pbeg + 1);
-    if (pbeg < pend) {
-        load(id);
-        scale_of(id, sk, sv);
+    const int np = pend - pbeg;
+    float sk = 0.f, ls = 0.f, skn = 0.f, lsn = 0.f;
+    if (np > 0) {
+        fetch(pbeg);
+        load(__builtin_amdgcn_readlane(lid, 0));
         store(page);
-        if (pbeg + 1 < pend) {
-            load(idn);
-            scale_of(idn, skn, svn);
-        }
+        sk = lane_f(lsk, 0);
+        ls = lane_f(lls, 0);
+        load(__builtin_amdgcn_readlane(lid, np > 1 ? 1 : 0));
+        skn = lane_f(lsk, 1);
+        lsn = lane_f(lls, 1);
     }
-    for (int pg = pbeg; pg < pend; pg++) {
-        const uint4 * cur = page + ((pg - pbeg) & 1) * FRAGS * 64;
-        __syncthreads();                                         // cur is whole, the other buffer is read
-        const float skc = sk, svc = sv;
-        if (pg + 1 < pend) {
-            store(page + ((pg + 1 - pbeg) & 1) * FRAGS * 64);
-            sk = skn;
-            sv = svn;
-            if (pg + 2 < pend) {
-                const int id2 = page_id(pg + 2);
-                load(id2);
-                scale_of(id2, skn, svn);
+    for (int n = 0; n < np; n++) {
+        const int t0 = (pbeg + n) * KV8_PAGE, n2 = n + 2;
+        const uint4 * cur = page + (n & 1) * FRAGS * 64;
+        const float skc = sk;
+        float lsc = ls;
+        if ((n2 & 63) == 0 && n2 < np) fetch(pbeg + n2);
+        lds_barrier();                                           // cur is whole, the other buffer is read
+        const bool skip = !live || t0 >= wlast.hi || t0 + KV8_PAGE <= wfirst.lo;
+        f32x16 sc[2];
+        if (!skip) {
+            // fragments four products ahead of their use, held in this order (the scheduler would read each just before it)
+            uint4 fr[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) fr[k] = cur[k * 64 + lane];
+#pragma unroll
+            for (int T = 0; T < 2; T++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) sc[T][e] = 0.f;
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < 2 * NC; k++) {
+                sc[k / NC] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, fr[k & 3]), q[k % NC], sc[k / NC], 0, 0, 0);
+                if (k + 4 < 2 * NC) fr[k & 3] = cur[(k + 4) * 64 + lane];
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
-        const int t0 = pg * KV8_PAGE;
-        if (!live || t0 >= wlast.hi || t0 + KV8_PAGE <= wfirst.lo) continue;
-        f32x16 sc[2];
-#pragma unroll
-        for (int T = 0; T < 2; T++) {
-#pragma unroll
-            for (int e = 0; e < 16; e++) sc[T][e] = 0.f;
-#pragma unroll
-            for (int k = 0; k < NC; k++)
-                sc[T] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, cur[(T * NC + k) * 64 + lane]), q[k], sc[T], 0, 0, 0);
+        if (n + 1 < np) {
+            store(page + (~n & 1) * FRAGS * 64);
+            sk = skn;
+            ls = lsn;
+            if (n2 < np) {
+                load(__builtin_amdgcn_readlane(lid, n2 & 63));
+                skn = lane_f(lsk, n2 & 63);
+                lsn = lane_f(lls, n2 & 63);
+            }
         }
+        if (skip) continue;
         const float cs0 = rowf * skc, cs = cs0 < 1e-35f ? 1e-35f : cs0;      // (above 0, so that -inf stays -inf; a NaN stays)
         const bool edge = t0 < wlast.lo || t0 + KV8_PAGE > wfirst.hi || t0 < lo || t0 + KV8_PAGE > hi;
         if (MASK) {
@@ -804,19 +833,18 @@ __global__ __launch_bounds__(KT, NC <= 8 ? 2 : 1) void k_kv8_tile(Kv8AttnArgs a)
         }
         if (!MASK) mx *= cs;
         // V's scale as a power of two within 2^4 of the reference, which moves otherwise (never 2^60 below the largest)
-        float ls = __builtin_amdgcn_logf(svc < 1e-36f ? 1e-36f : svc);       // log2; of a NaN NaN
-        const bool poison = !(ls < 128.f);
-        if (poison) ls = eref > -1000 ? (float) eref : 0.f;
+        const bool poison = !(lsc < 128.f);
+        if (poison) lsc = eref > -1000 ? (float) eref : 0.f;
         const float step = MASK ? 3.f / LOG2E : 3.f;
         const bool move = mx > m + step || (m == -inf && mx > m);
-        const bool shift = fabsf(ls - (float) eref) > 4.f;
+        const bool shift = fabsf(lsc - (float) eref) > 4.f;
         if (__any(move) || shift) {
             const float mn = move ? mx : m, base = mn == -inf ? 0.f : mn;
             float f = m == -inf ? 0.f : __builtin_amdgcn_exp2f(MASK ? (m - base) * LOG2E : m - base);
             l *= f;
             m = mn;
             if (shift) {
-                int e = (int) rintf(ls);
+                int e = (int) rintf(lsc);
                 emax = e > emax ? e : emax;
                 e = e < emax - 60 ? emax - 60 : e;
                 f = ldexpf(f, eref - e > 200 ? 200 : (eref - e < -200 ? -200 : eref - e));
@@ -828,7 +856,7 @@ __global__ __launch_bounds__(KT, NC <= 8 ? 2 : 1) void k_kv8_tile(Kv8AttnArgs a)
                 for (int e = 0; e < 16; e++) o[t][e] *= f;
         }
         // weights: 2^8 e^(x - m) sv 2^-eref in fp16
-        const float base = m == -inf ? 0.f : m, lr = 8.f + (ls - (float) eref);
+        const float base = m == -inf ? 0.f : m, lr = 8.f + (lsc - (float) eref);
         float k = cs, off = lr - base;
         if (!MASK && __any(fabsf(base) > 65536.f)) {             // there a score's own rounding counts, as m has it
 #pragma unroll
@@ -961,24 +989,30 @@ __global__ __launch_bounds__(KT) void k_kv8_combine(Kv8AttnArgs a) {
 }
 
 // tile: k_kv8_tile's plan, else k_kv8_step's
-struct AttnPlan { bool tile; int RS, ngrp, C, nch, fold; };
+struct AttnPlan { bool tile; int RS, ngrp, C, nch, fold, wv; };
 
-AttnPlan attn_plan(int f32, int Hq, int Hkv, int nseq, int max_n, int max_len, int window) {
+AttnPlan attn_plan(int f32, int Hq, int D, int Hkv, int nseq, int max_n, int max_len, int window) {
     AttnPlan p;
     const int64_t rows = (int64_t) max_n * (Hq / Hkv);
     p.tile = !f32 && rows > 16;
     p.RS = rows <= 4 ? 1 : (rows <= 8 ? 2 : 4);
-    const int group = p.tile ? TR : 4 * p.RS;
+    p.wv = D <= 64 || (D > 96 && D <= 128) ? 8 : 4;
+    if (getenv("X_WV") && D <= 128) p.wv = atoi(getenv("X_WV"));
+    const int group = p.tile ? 32 * p.wv : 4 * p.RS;
     p.ngrp = (int) ((rows + group - 1) / group);
     const int64_t wgs = (int64_t) Hkv * p.ngrp * nseq, round = p.tile ? KV8_PAGE : SW * KV8_PAGE;
     // step: chunks of whole rounds of the waves; tile: enough workgroups for two a CU, chunks of 512 tokens or more
     int64_t nch = ((p.tile ? 512 : 1024) + wgs - 1) / wgs, most = (max_len + (p.tile ? 511 : round - 1)) / (p.tile ? 512 : round);
+    const int slots = 256 * 8 / p.wv;
+    if (p.tile && wgs < slots) nch = slots / wgs;
+    if (p.tile && getenv("X_NCH")) nch = atoi(getenv("X_NCH"));
     if (nch > most) nch = most;
     int64_t C = (max_len + nch - 1) / nch;
     C = (C + round - 1) / round * round;
     p.C = (int) (C > (1 << 30) ? 1 << 30 : C);
     p.nch = (int) ((max_len + (int64_t) p.C - 1) / p.C);
     p.fold = wgs * p.nch <= 512;
+    if (getenv("X_FOLD")) p.fold = atoi(getenv("X_FOLD"));
     return p;
 }
 
@@ -994,8 +1028,14 @@ template <int NC> hipError_t run_attn(const Kv8AttnArgs & a, const AttnPlan & p,
     if (!p.tile) return p.RS == 1 ? run_step<NC, 1>(a, p, s) : (p.RS == 2 ? run_step<NC, 2>(a, p, s) : run_step<NC, 4>(a, p, s));
     const dim3 grid((unsigned) (a.c.Hkv * p.ngrp), (unsigned) p.nch, (unsigned) a.t.nseq);
     const size_t lds = 2 * 4 * NC * 1024;
-    if (a.mask) k_kv8_tile<NC, true><<<grid, KT, lds, s>>>(a);
-    else k_kv8_tile<NC, false><<<grid, KT, lds, s>>>(a);
+    if constexpr (NC <= 8 && NC % 4 == 0)
+        if (p.wv == 8) {
+            if (a.mask) k_kv8_tile<NC, 8, true><<<grid, 512, lds, s>>>(a);
+            else k_kv8_tile<NC, 8, false><<<grid, 512, lds, s>>>(a);
+            return hipGetLastError();
+        }
+    if (a.mask) k_kv8_tile<NC, 4, true><<<grid, KT, lds, s>>>(a);
+    else k_kv8_tile<NC, 4, false><<<grid, KT, lds, s>>>(a);
     return hipGetLastError();
 }
 
@@ -1027,14 +1067,14 @@ hipError_t launch_kv8_read(const Kv8Cache & c, const Kv8Table & t, void * k, voi
 }
 
 int64_t kv8_attn_ws_bytes(int f32, int Hq, int D, int Hkv, int nseq, int64_t T, int max_n, int max_len, int window) {
-    const AttnPlan p = attn_plan(f32, Hq, Hkv, nseq, max_n, max_len, window);
+    const AttnPlan p = attn_plan(f32, Hq, D, Hkv, nseq, max_n, max_len, window);
     return p.nch == 1 ? 0 : T * Hq * p.nch * (D + 2) * (int64_t) sizeof(float);
 }
 
 hipError_t launch_kv8_attn(const Kv8Cache & c, const Kv8Table & t, const void * q, int f32, int Hq, int64_t qrs, int64_t qhs,
                            int max_len, const float * mask, int64_t mld, const float * sinks, int window, float scale,
                            void * out, void * ws, hipStream_t s) {
-    const AttnPlan p = attn_plan(f32, Hq, c.Hkv, t.nseq, t.max_n, max_len, window);
+    const AttnPlan p = attn_plan(f32, Hq, c.D, c.Hkv, t.nseq, t.max_n, max_len, window);
     Kv8AttnArgs a{c, t, q, out, mask, sinks, (float *) ws, qrs, qhs, mld, scale, Hq, Hq / c.Hkv, max_len, window, f32, p.C, p.nch, p.fold};
     if (!grid_fits((int64_t) Hq * t.max_n, t.nseq) || !grid_fits((int64_t) c.Hkv * p.ngrp, t.nseq) || p.nch > 65535)
         return hipErrorInvalidValue;
