@@ -630,13 +630,15 @@ __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-template <int NC, int WV, bool MASK>
+template <int NC, int WV, int KS, bool MASK>
 __global__ __launch_bounds__(64 * WV, NC <= 8 ? 8 / WV : 1) void k_kv8_tile(Kv8AttnArgs a) {
-    constexpr int NU = 2 * NC / WV, ND = NC / 2, FRAGS = 4 * NC, TR = 32 * WV;       // load units of a wave, d tiles of 32, KiB of a
-                                                                                     // page, rows of a workgroup
-    static_assert(NU * WV == 2 * NC, "the waves share a page's units evenly");
-    extern __shared__ __align__(16) uint4 page[];                // [2][FRAGS][64]
-    const int D = a.c.D, nc = D / 16, lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    constexpr int WR = WV / KS, TR = 32 * WR, NU = 2 * NC / WR, ND = NC / 2;         // waves over the rows, rows, a wave's load
+    constexpr int FRAGS = 4 * NC;                                                    // units, d tiles of 32, KiB of a page
+    static_assert(NU * WR == 2 * NC, "the waves share a page's units evenly");
+    extern __shared__ __align__(16) uint4 lds4[];                // [KS][2][FRAGS][64]
+    const int D = a.c.D, nc = D / 16, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int w = wave % WR, grp = wave / WR;                    // of KS groups of waves, each with every KS-th page
+    uint4 * page = lds4 + grp * 2 * FRAGS * 64;
     const int c = blockIdx.y, i = blockIdx.z, half = lane >> 5, n31 = lane & 31;
     const int g = blockIdx.x % a.c.Hkv;
     int z = blockIdx.x / a.c.Hkv;
@@ -663,7 +665,7 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 ? 8 / WV : 1) void k_kv8_tile(Kv8A
     int src[NU], dst[NU][2];
 #pragma unroll
     for (int u = 0; u < NU; u++) {
-        const int k = w + WV * u;
+        const int k = w + WR * u;
         if (k < NC) {                                            // K: tokens 32 T + n31, chunk 2 s + half
             const int T = k / (NC / 2), s2 = k % (NC / 2), ch = 2 * s2 + half < nc ? 2 * s2 + half : nc - 1;
             src[u] = ((2 * T + (n31 >> 4)) * nc + ch) * 256 + (lane & 15) * 16;
@@ -698,7 +700,7 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 ? 8 / WV : 1) void k_kv8_tile(Kv8A
     int lid = 0;
     float lsk = 0.f, lls = 0.f;               // K's scale, log2 of V's
     auto fetch = [&](int p0) {
-        const int id = p0 + lane < pend ? kv8_page(tab, p0 + lane, a.t.P, a.c.pages) : -1;
+        const int at = p0 + KS * lane, id = at < pend ? kv8_page(tab, at, a.t.P, a.c.pages) : -1;
         const float * p = a.c.scales + ((int64_t) (id < 0 ? 0 : id) * a.c.Hkv + g) * 2;
         const bool bad = id < 0 || full > a.max_len;
         lid = id < 0 ? 0 : id;
@@ -706,6 +708,17 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 ? 8 / WV : 1) void k_kv8_tile(Kv8A
         lls = bad ? nan : __builtin_amdgcn_logf(p[1] < 1e-36f ? 1e-36f : p[1]);
     };
     auto lane_f = [&](float v, int n) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), n)); };
+
+    const int p0 = pbeg + grp, np = pend > p0 ? (pend - p0 + KS - 1) / KS : 0, rounds = pend > pbeg ? (pend - pbeg + KS - 1) / KS : 0;
+    float sk = 0.f, ls = 0.f, skn = 0.f, lsn = 0.f;
+    if (np > 0) {                             // (the first page's codes are on their way while q is prepared)
+        fetch(p0);
+        load(__builtin_amdgcn_readlane(lid, 0));
+        sk = lane_f(lsk, 0);
+        ls = lane_f(lls, 0);
+        skn = lane_f(lsk, 1);
+        lsn = lane_f(lls, 1);
+    }
 
     // this lane's row
     const int rr = w * 32 + n31 < nrow ? w * 32 + n31 : nrow - 1, j = (R0 + rr) / a.rep, h = g * a.rep + (R0 + rr - j * a.rep);
@@ -750,26 +763,18 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 ? 8 / WV : 1) void k_kv8_tile(Kv8A
     float m = -inf, l = 0.f;
     int eref = -1000, emax = -1000;                              // no page yet
 
-    const int np = pend - pbeg;
-    float sk = 0.f, ls = 0.f, skn = 0.f, lsn = 0.f;
     if (np > 0) {
-        fetch(pbeg);
-        load(__builtin_amdgcn_readlane(lid, 0));
         store(page);
-        sk = lane_f(lsk, 0);
-        ls = lane_f(lls, 0);
         load(__builtin_amdgcn_readlane(lid, np > 1 ? 1 : 0));
-        skn = lane_f(lsk, 1);
-        lsn = lane_f(lls, 1);
     }
-    for (int n = 0; n < np; n++) {
-        const int t0 = (pbeg + n) * KV8_PAGE, n2 = n + 2;
+    for (int n = 0; n < rounds; n++) {
+        const int t0 = (p0 + n * KS) * KV8_PAGE, n2 = n + 2;
         const uint4 * cur = page + (n & 1) * FRAGS * 64;
         const float skc = sk;
         float lsc = ls;
-        if ((n2 & 63) == 0 && n2 < np) fetch(pbeg + n2);
+        if ((n2 & 63) == 0 && n2 < np) fetch(p0 + n2 * KS);
         lds_barrier();                                           // cur is whole, the other buffer is read
-        const bool skip = !live || t0 >= wlast.hi || t0 + KV8_PAGE <= wfirst.lo;
+        const bool skip = !live || n >= np || t0 >= wlast.hi || t0 + KV8_PAGE <= wfirst.lo;
         f32x16 sc[2];
         if (!skip) {
             // fragments four products ahead of their use, held in this order (the scheduler would read each just before it)
@@ -899,6 +904,39 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 ? 8 / WV : 1) void k_kv8_tile(Kv8A
                         __builtin_bit_cast(f16x8, cur[(2 * NC + t * 4 + T * 2 + v) * 64 + lane]), b, o[t], 0, 0, 0);
             }
     }
+    if (KS > 1) {                             // the groups meet in the first, through LDS, in units of 2^m and 2^eref
+        lds_barrier();
+        float * ex = (float *) lds4 + w * (16 * ND + 2) * 64 + lane;
+        const float unit = MASK ? LOG2E : 1.f;
+#pragma unroll
+        for (int k = 1; k < KS; k++) {
+            if (grp == k && live) {
+                const float f = ldexpf(1.f, eref <= -1000 ? 0 : eref);
+                ex[0] = m;
+                ex[64] = l;
+#pragma unroll
+                for (int t = 0; t < ND; t++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) ex[(2 + 16 * t + e) * 64] = o[t][e] * f;
+            }
+            lds_barrier();
+            if (grp == 0 && live) {
+                const float mo = ex[0], lo2 = ex[64], mn = fmaxf(m, mo), base = mn == -inf ? 0.f : mn;
+                float f = __builtin_amdgcn_exp2f((m - base) * unit);
+                const float fo = __builtin_amdgcn_exp2f((mo - base) * unit);
+                l = l * f + lo2 * fo;
+                f = ldexpf(f, eref <= -1000 ? 0 : eref);
+#pragma unroll
+                for (int t = 0; t < ND; t++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) o[t][e] = fmaf(o[t][e], f, ex[(2 + 16 * t + e) * 64] * fo);
+                m = mn;
+                eref = 0;
+            }
+            if (k + 1 < KS) lds_barrier();
+        }
+        if (grp > 0) return;
+    }
     if (!live || w * 32 + n31 >= nrow) return;
     {
         typedef unsigned u2 __attribute__((ext_vector_type(2)));
@@ -922,12 +960,12 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 ? 8 / WV : 1) void k_kv8_tile(Kv8A
     for (int t = 0; t < ND; t++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
+            if (32 * t + 8 * e >= D) continue;
             const int d = 32 * t + 8 * e + 4 * half;
-            if (d >= D) continue;
             const float4 y = make_float4(o[t][4 * e] * f, o[t][4 * e + 1] * f, o[t][4 * e + 2] * f, o[t][4 * e + 3] * f);
             if (a.nch > 1) *(float4 *) (a.ws + (at * a.nch + c) * D + d) = y;
             else *(uint2 *) ((uint16_t *) a.out + at * D + d) =
-                make_uint2(f32_to_bf16(y.x) | (uint32_t) f32_to_bf16(y.y) << 16, f32_to_bf16(y.z) | (uint32_t) f32_to_bf16(y.w) << 16);
+                make_uint2(pack_bf16(y.x, y.y), pack_bf16(y.z, y.w));
         }
 }
 
@@ -989,7 +1027,7 @@ __global__ __launch_bounds__(KT) void k_kv8_combine(Kv8AttnArgs a) {
 }
 
 // tile: k_kv8_tile's plan, else k_kv8_step's
-struct AttnPlan { bool tile; int RS, ngrp, C, nch, fold, wv; };
+struct AttnPlan { bool tile; int RS, ngrp, C, nch, fold, wv, ks; };
 
 AttnPlan attn_plan(int f32, int Hq, int D, int Hkv, int nseq, int max_n, int max_len, int window) {
     AttnPlan p;
@@ -997,12 +1035,15 @@ AttnPlan attn_plan(int f32, int Hq, int D, int Hkv, int nseq, int max_n, int max
     p.tile = !f32 && rows > 16;
     p.RS = rows <= 4 ? 1 : (rows <= 8 ? 2 : 4);
     p.wv = D <= 64 || (D > 96 && D <= 128) ? 8 : 4;
+    p.ks = p.wv == 8 ? 2 : 1;
     if (getenv("X_WV") && D <= 128) p.wv = atoi(getenv("X_WV"));
-    const int group = p.tile ? 32 * p.wv : 4 * p.RS;
+    if (getenv("X_KS")) p.ks = atoi(getenv("X_KS"));
+    if (p.wv == 4) p.ks = 1;
+    const int group = p.tile ? 32 * p.wv / p.ks : 4 * p.RS;
     p.ngrp = (int) ((rows + group - 1) / group);
     const int64_t wgs = (int64_t) Hkv * p.ngrp * nseq, round = p.tile ? KV8_PAGE : SW * KV8_PAGE;
     // step: chunks of whole rounds of the waves; tile: enough workgroups for two a CU, chunks of 512 tokens or more
-    int64_t nch = ((p.tile ? 512 : 1024) + wgs - 1) / wgs, most = (max_len + (p.tile ? 511 : round - 1)) / (p.tile ? 512 : round);
+    int64_t nch = p.tile ? 1 : (1024 + wgs - 1) / wgs, most = (max_len + (p.tile ? 511 : round - 1)) / (p.tile ? 512 : round);
     const int slots = 256 * 8 / p.wv;
     if (p.tile && wgs < slots) nch = slots / wgs;
     if (p.tile && getenv("X_NCH")) nch = atoi(getenv("X_NCH"));
@@ -1030,12 +1071,14 @@ template <int NC> hipError_t run_attn(const Kv8AttnArgs & a, const AttnPlan & p,
     const size_t lds = 2 * 4 * NC * 1024;
     if constexpr (NC <= 8 && NC % 4 == 0)
         if (p.wv == 8) {
-            if (a.mask) k_kv8_tile<NC, 8, true><<<grid, 512, lds, s>>>(a);
-            else k_kv8_tile<NC, 8, false><<<grid, 512, lds, s>>>(a);
+            if (p.ks == 2 && a.mask) k_kv8_tile<NC, 8, 2, true><<<grid, 512, 2 * lds, s>>>(a);
+            else if (p.ks == 2) k_kv8_tile<NC, 8, 2, false><<<grid, 512, 2 * lds, s>>>(a);
+            else if (a.mask) k_kv8_tile<NC, 8, 1, true><<<grid, 512, lds, s>>>(a);
+            else k_kv8_tile<NC, 8, 1, false><<<grid, 512, lds, s>>>(a);
             return hipGetLastError();
         }
-    if (a.mask) k_kv8_tile<NC, 4, true><<<grid, KT, lds, s>>>(a);
-    else k_kv8_tile<NC, 4, false><<<grid, KT, lds, s>>>(a);
+    if (a.mask) k_kv8_tile<NC, 4, 1, true><<<grid, KT, lds, s>>>(a);
+    else k_kv8_tile<NC, 4, 1, false><<<grid, KT, lds, s>>>(a);
     return hipGetLastError();
 }
 

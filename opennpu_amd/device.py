@@ -249,30 +249,47 @@ def kv8_cache(pages, Hkv, D, device=None):
             torch.zeros((pages, Hkv, 2), dtype=torch.float32, device=device or "cuda"))
 
 
-def _kv8(codes, scales, table, pos, off, vals, what):
-    """the cache's, table's and row ranges' arguments, checked; vals: (fp32 or bf16 [T][heads][D] tensor, ...)"""
+def _kv8_refuse(codes, scales, table, pos, off, vals, what, here):
+    """the reason why _kv8 does not take its arguments"""
     import torch
-    pages, Hkv, two, w = codes.shape
-    D = w // 64
-    if codes.dtype != torch.int8 or two != 2 or w % 64 or not codes.is_contiguous():
+    if codes.dtype != torch.int8 or codes.dim() != 4 or codes.shape[2] != 2 or codes.shape[3] % 64 or not codes.is_contiguous():
         raise ValueError(f"{what}: codes must be int8 [pages][Hkv][2][64 D], contiguous")
     if scales.dtype != torch.float32 or scales.shape != codes.shape[:3] or not scales.is_contiguous():
         raise ValueError(f"{what}: scales must be fp32 [pages][Hkv][2], contiguous")
-    nseq, P = table.shape
-    if table.dtype != torch.int32 or (P > 1 and table.stride(1) != 1):
+    if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
         raise ValueError(f"{what}: table must be int32 [sequences][P] with rows of unit stride")
-    if pos.dtype != torch.int32 or pos.shape != (nseq,) or not pos.is_contiguous():
+    if pos.dtype != torch.int32 or pos.shape != table.shape[:1] or not pos.is_contiguous():
         raise ValueError(f"{what}: positions or lengths must be int32, one per sequence, contiguous")
-    if off is not None and (off.dtype != torch.int32 or off.shape != (nseq + 1,) or not off.is_contiguous()):
+    if off is not None and (off.dtype != torch.int32 or off.shape != (table.shape[0] + 1,) or not off.is_contiguous()):
         raise ValueError(f"{what}: off must be int32, one more than the sequences, contiguous")
-    here = torch.cuda.current_device()
     for t in (codes, scales, table, pos, off) + vals:
         if t is not None and not (t.is_cuda and t.get_device() == here):
             raise ValueError(f"{what}: every tensor must be on the current GPU (cuda:{here}), got {t.device}")
+    raise ValueError(f"{what}: rows must be fp32 or bf16 [T][heads][{codes.shape[3] // 64}] with unit stride in the last dimension")
+
+
+def _kv8(codes, scales, table, pos, off, vals, what):
+    """the cache's, table's and row ranges' arguments, checked (in one expression: a decode step's call is bound
+    by its issue); vals: (fp32 or bf16 [T][heads][D] tensor, ...). Returns pages, Hkv, D, sequences, P, the GPU"""
+    import torch
+    f32, i32, bf16 = torch.float32, torch.int32, torch.bfloat16
+    here = torch.cuda.current_device()
+    cs, ts = codes.shape, table.shape
+    ok = (codes.dtype is torch.int8 and len(cs) == 4 and cs[2] == 2 and cs[3] % 64 == 0 and scales.dtype is f32
+          and scales.shape == cs[:3] and table.dtype is i32 and len(ts) == 2 and (ts[1] <= 1 or table.stride(1) == 1)
+          and pos.dtype is i32 and pos.shape == ts[:1] and codes.is_contiguous() and scales.is_contiguous()
+          and pos.is_contiguous() and codes.get_device() == here == scales.get_device() == table.get_device() == pos.get_device())
+    if off is not None:
+        ok = ok and off.dtype is i32 and off.shape == (ts[0] + 1,) and off.is_contiguous() and off.get_device() == here
+    D = cs[-1] // 64
     for t in vals:
-        if t.dim() != 3 or t.shape[2] != D or t.stride(2) != 1 or t.dtype not in (torch.float32, torch.bfloat16):
-            raise ValueError(f"{what}: rows must be fp32 or bf16 [T][heads][{D}] with unit stride in the last dimension")
-    return pages, Hkv, D, nseq, P
+        if not ok:
+            break
+        shape = t.shape
+        ok = len(shape) == 3 and shape[2] == D and t.stride(2) == 1 and t.get_device() == here and (t.dtype is f32 or t.dtype is bf16)
+    if not ok:
+        _kv8_refuse(codes, scales, table, pos, off, vals, what, here)
+    return cs[0], cs[1], D, ts[0], ts[1], here
 
 
 def _kv8_n(T, nseq, off, max_n, what):
@@ -284,20 +301,27 @@ def _kv8_n(T, nseq, off, max_n, what):
     return T if max_n is None else int(max_n)
 
 
+def _raw_stream(here):
+    import torch
+    return torch._C._cuda_getCurrentRawStream(here)
+
+
 def kv8_write(codes, scales, k, v, table, pos, off=None, max_n=None):
     """Quantise k, v (fp32 or bf16 [T][Hkv][D]) into the cache's pages (onpu_kv8_write_dev): sequence i's
     rows off[i]:off[i + 1] (off None: T / sequences each) go to positions pos[i], pos[i] + 1, ...; max_n: the most
     rows of one sequence (default: as many as there are)."""
     import torch
     L = require_gpu()
-    pages, Hkv, D, nseq, P = _kv8(codes, scales, table, pos, off, (k, v), "kv8_write")
-    if k.shape != v.shape or k.dtype != v.dtype or k.shape[1] != Hkv:
+    pages, Hkv, D, nseq, P, here = _kv8(codes, scales, table, pos, off, (k, v), "kv8_write")
+    T, heads, _ = k.shape
+    if k.shape != v.shape or k.dtype is not v.dtype or heads != Hkv:
         raise ValueError("kv8_write: k and v must have the same type and shape [T][Hkv][D]")
-    T = k.shape[0]
-    check(L.onpu_kv8_write_dev(_ptr(codes), _ptr(scales), pages, Hkv, D, _ptr(k), _ptr(v), int(k.dtype == torch.bfloat16),
-                               k.stride(0), k.stride(1), v.stride(0), v.stride(1), _ptr(table), table.stride(0), P,
-                               _ptr(pos), None if off is None else _ptr(off), nseq, T,
-                               _kv8_n(T, nseq, off, max_n, "kv8_write"), _stream()), "kv8_write")
+    krs, khs, _ = k.stride()
+    vrs, vhs, _ = v.stride()
+    check(L.onpu_kv8_write_dev(codes.data_ptr(), scales.data_ptr(), pages, Hkv, D, k.data_ptr(), v.data_ptr(),
+                               k.dtype is torch.bfloat16, krs, khs, vrs, vhs, table.data_ptr(), table.stride(0), P,
+                               pos.data_ptr(), None if off is None else off.data_ptr(), nseq, T,
+                               _kv8_n(T, nseq, off, max_n, "kv8_write"), _raw_stream(here)), "kv8_write")
 
 
 def kv8_read(codes, scales, table, pos, rows, off=None, max_n=None, dtype=None, out=None):
@@ -305,19 +329,22 @@ def kv8_read(codes, scales, table, pos, rows, off=None, max_n=None, dtype=None, 
     [rows][Hkv][D], bf16 (the default) or fp32; rows in all, off and max_n as kv8_write."""
     import torch
     L = require_gpu()
-    pages, Hkv, D, nseq, P = _kv8(codes, scales, table, pos, off, tuple(out or ()), "kv8_read")
+    pages, Hkv, D, nseq, P, here = _kv8(codes, scales, table, pos, off, () if out is None else tuple(out), "kv8_read")
     if out is None:
-        k, v = (torch.empty((rows, Hkv, D), dtype=dtype or torch.bfloat16, device=codes.device) for _ in range(2))
-        if k.dtype not in (torch.float32, torch.bfloat16):
+        dtype = dtype or torch.bfloat16
+        if dtype is not torch.float32 and dtype is not torch.bfloat16:
             raise ValueError("kv8_read: dtype must be fp32 or bf16")
+        k = codes.new_empty((rows, Hkv, D), dtype=dtype)
+        v = torch.empty_like(k)
     else:
         k, v = out
         if k.shape != (rows, Hkv, D) or v.shape != k.shape or k.dtype != v.dtype or not (k.is_contiguous() and v.is_contiguous()) \
                 or dtype not in (None, k.dtype):
             raise ValueError("kv8_read: out must be two contiguous [rows][Hkv][D] tensors of one type")
-    check(L.onpu_kv8_read_dev(_ptr(codes), _ptr(scales), pages, Hkv, D, _ptr(table), table.stride(0), P, _ptr(pos),
-                              None if off is None else _ptr(off), nseq, rows, _kv8_n(rows, nseq, off, max_n, "kv8_read"),
-                              _ptr(k), _ptr(v), int(k.dtype == torch.bfloat16), _stream()), "kv8_read")
+    check(L.onpu_kv8_read_dev(codes.data_ptr(), scales.data_ptr(), pages, Hkv, D, table.data_ptr(), table.stride(0), P,
+                              pos.data_ptr(), None if off is None else off.data_ptr(), nseq, rows,
+                              _kv8_n(rows, nseq, off, max_n, "kv8_read"), k.data_ptr(), v.data_ptr(),
+                              k.dtype is torch.bfloat16, _raw_stream(here)), "kv8_read")
     return k, v
 
 
@@ -327,28 +354,34 @@ def kv8_attn(q, codes, scales, table, lens, off=None, max_n=None, max_len=None, 
     rows off[i]:off[i + 1] (off None: T / sequences each) of sequence i's lens[i] cached tokens. max_n, max_len: the most query rows
     and tokens of one sequence (default: as many as there are, and as the table holds; closer bounds run
     faster). mask fp32 [sequences][>= max_len] is added to the scores, sinks fp32 [Hq] is a logit per head without a
-    value, window the last positions a query sees (0: all). Returns out [T][Hq][D] in q's type."""
+    value, window the last positions a query sees (0: all). ws: a workspace of onpu_kv8_attn_ws_bytes bytes, one
+    per call in flight (default: torch's allocator). Returns out [T][Hq][D] in q's type."""
     import torch
     L = require_gpu()
-    pages, Hkv, D, nseq, P = _kv8(codes, scales, table, lens, off, (q,) if out is None else (q, out), "kv8_attn")
-    T, Hq = q.shape[0], q.shape[1]
+    pages, Hkv, D, nseq, P, here = _kv8(codes, scales, table, lens, off, (q,) if out is None else (q, out), "kv8_attn")
+    T, Hq, _ = q.shape
+    qrs, qhs, _ = q.stride()
+    bf16 = q.dtype is torch.bfloat16
     n = _kv8_n(T, nseq, off, max_n, "kv8_attn")
     max_len = 64 * P if max_len is None else int(max_len)
     if out is None:
-        out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
         raise ValueError("kv8_attn: out must be contiguous, of q's shape and type")
     for t, shape in ((mask, None), (sinks, (Hq,))):
-        if t is not None and (t.dtype != torch.float32 or not t.is_cuda or t.get_device() != q.get_device() or t.stride(-1) != 1
+        if t is not None and (t.dtype != torch.float32 or t.get_device() != here or t.stride(-1) != 1
                               or (t.shape != shape if shape else t.dim() != 2 or t.shape[0] != nseq or t.shape[1] < max_len)):
             raise ValueError("kv8_attn: mask must be fp32 [sequences][>= max_len], sinks fp32 [Hq], on q's GPU")
-    nb = L.onpu_kv8_attn_ws_bytes(int(q.dtype == torch.bfloat16), Hq, D, Hkv, nseq, T, n, max_len, window)
-    if nb and ws is None:
-        ws = torch.empty((nb,), dtype=torch.uint8, device=q.device)
-    check(L.onpu_kv8_attn_dev(_ptr(q), int(q.dtype == torch.bfloat16), Hq, q.stride(0), q.stride(1), _ptr(codes),
-                              _ptr(scales), pages, Hkv, D, _ptr(table), table.stride(0), P, _ptr(lens),
-                              None if off is None else _ptr(off), nseq, T, n, max_len, None if mask is None else _ptr(mask),
-                              0 if mask is None else mask.stride(0), None if sinks is None else _ptr(sinks), int(window),
-                              float(D ** -0.5 if scale is None else scale), _ptr(out), None if ws is None else _ptr(ws),
-                              0 if ws is None else ws.nbytes, _stream()), "kv8_attn")
+    if ws is None:
+        nb = L.onpu_kv8_attn_ws_bytes(bf16, Hq, D, Hkv, nseq, T, n, max_len, window)
+        if nb:
+            ws = codes.new_empty((nb,))
+    elif ws.get_device() != here or not ws.is_contiguous():
+        raise ValueError("kv8_attn: ws must be contiguous, on q's GPU")
+    check(L.onpu_kv8_attn_dev(q.data_ptr(), bf16, Hq, qrs, qhs, codes.data_ptr(), scales.data_ptr(), pages, Hkv, D,
+                              table.data_ptr(), table.stride(0), P, lens.data_ptr(), None if off is None else off.data_ptr(),
+                              nseq, T, n, max_len, None if mask is None else mask.data_ptr(),
+                              0 if mask is None else mask.stride(0), None if sinks is None else sinks.data_ptr(), window,
+                              D ** -0.5 if scale is None else scale, out.data_ptr(), None if ws is None else ws.data_ptr(),
+                              0 if ws is None else ws.nbytes, _raw_stream(here)), "kv8_attn")
     return out
