@@ -321,6 +321,24 @@ __device__ __forceinline__ float wave_sum(float v) {
 }
 constexpr float LOG2E = 1.44269504088896341f;
 
+// a workgroup barrier that orders LDS accesses only: global loads stay in flight across it
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// values [at, at + 4) of a page's mask, of which the first `have` exist (uniform); 0 for the others
+__device__ __forceinline__ f32x4 mask4(const float * page, int at, int have) {
+    struct __attribute__((packed, aligned(4))) V { f32x4 v; };   // (rows start anywhere)
+    if (have >= KV8_PAGE) return ((const V *) (page + at))->v;
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void *) page, (short) 0, 4 * have, 0x00020000);
+    f32x4 v;
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, 4 * (at + e), 0, 0));
+    return v;
+}
+
 // the larger (or the sum) of x and the lane 32, then 16 away
 template <bool MAX> __device__ __forceinline__ float across_quads(float x) {
     typedef unsigned u2 __attribute__((ext_vector_type(2)));
@@ -344,11 +362,10 @@ __device__ __forceinline__ float quad_sum(float x) {
 // product's operand without a move across lanes. A wave takes every fourth page, K of its next one loading
 // once this one's scores are out, V after its products; waves meet in LDS, chunks in k_kv8_combine.
 // RS sets of 4 rows; NC: chunks of 16 d (D / 16 or more).
-constexpr int SW = KT / 64;                   // waves
-template <int NC, int RS, bool MASK>
-__global__ __launch_bounds__(KT) void k_kv8_step(Kv8AttnArgs a) {
+template <int NC, int RS, int SW, bool MASK>
+__global__ __launch_bounds__(64 * SW, SW == 8 ? 2 : (RS == 1 ? (NC <= 4 ? 4 : (NC <= 8 ? 3 : (NC <= 12 ? 2 : 1))) : (RS * NC <= 16 ? 2 : 1))) void k_kv8_step(Kv8AttnArgs a) {
     constexpr int KS = (NC + 3) / 4, HG = 4 * RS;
-    extern __shared__ __align__(16) float lds[];                 // red [SW][HG][D], ml [SW][HG][2]
+    extern __shared__ __align__(16) float lds[];                 // red [SW][HG][D], ml [SW][HG][2], the rows' bytes for RS > 1
     const int D = a.c.D, nc = D / 16, lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = blockIdx.x % a.c.Hkv, z = blockIdx.x / a.c.Hkv, c = blockIdx.y, i = blockIdx.z;
     const int quad = lane >> 4, part = lane & 3;
@@ -366,41 +383,37 @@ __global__ __launch_bounds__(KT) void k_kv8_step(Kv8AttnArgs a) {
     const int32_t * tab = a.t.table + i * a.t.tld;
     const float nan = __uint_as_float(0x7fc00000u);
 
-    // q, 16 values of a lane's row and step
-    float q[RS][KS][16];
-    int rlo[RS], rhi[RS];
-#pragma unroll
-    for (int k = 0; k < RS; k++) {
+    // a lane's row of set k: which positions it sees, where its q is
+    auto row_of = [&](int k, Kv8Seen & sees) {
         const int rr = 4 * k + ((lane & 15) >> 2) < nrow ? 4 * k + ((lane & 15) >> 2) : nrow - 1;
         const int R = R0 + rr, j = R / a.rep, h = g * a.rep + (R - j * a.rep);
-        const Kv8Seen s = kv8_seen(at0 + j, len, a.window);
-        rlo[k] = s.lo;
-        rhi[k] = s.hi;
-        const int64_t base = (r.row + j) * a.qrs + h * a.qhs;
+        sees = kv8_seen(at0 + j, len, a.window);
+        return (r.row + j) * a.qrs + h * a.qhs;
+    };
+    int rlo[RS], rhi[RS];
+    int64_t qat[RS];
 #pragma unroll
-        for (int s2 = 0; s2 < KS; s2++) {
-            const int d = 64 * s2 + 16 * quad;
-            if (a.f32) load16<true>(a.q, base + (d < D ? d : 0), q[k][s2]);
-            else load16<false>(a.q, base + (d < D ? d : 0), q[k][s2]);
-            if (d >= D)
-#pragma unroll
-                for (int e = 0; e < 16; e++) q[k][s2][e] = 0.f;
-        }
+    for (int k = 0; k < RS; k++) {
+        Kv8Seen sees;
+        qat[k] = row_of(k, sees);
+        rlo[k] = sees.lo;
+        rhi[k] = sees.hi;
     }
     uint4 kr[4][KS], vr[NC];
+    const uint32_t lane16 = 16 * lane;
     float sk, sv;
     auto page_base = [&](int id) { return a.c.codes + ((int64_t) (id < 0 ? 0 : id) * a.c.Hkv + g) * 2 * KV8_PAGE * D; };
     auto load_k = [&](int id) {               // (steps past D meet zeros of q; they read on into V's codes)
-        const int8_t * p = page_base(id) + 16 * lane;
+        const int8_t * p = page_base(id);     // (uniform: the lane's offset stays one register)
 #pragma unroll
         for (int t = 0; t < 4; t++)
 #pragma unroll
-            for (int s = 0; s < KS; s++) kr[t][s] = *(const uint4 *) (p + t * nc * 256 + s * 1024);
+            for (int s = 0; s < KS; s++) kr[t][s] = *(const uint4 *) (p + t * nc * 256 + s * 1024 + lane16);
     };
     auto load_v = [&](int id) {               // (chunks past D re-read the last: not stored)
-        const int8_t * p = page_base(id) + KV8_PAGE * D + 16 * lane;
+        const int8_t * p = page_base(id) + KV8_PAGE * D;
 #pragma unroll
-        for (int n = 0; n < NC; n++) vr[n] = *(const uint4 *) (p + (n < nc ? n : nc - 1) * 1024);
+        for (int n = 0; n < NC; n++) vr[n] = *(const uint4 *) (p + (n < nc ? n : nc - 1) * 1024 + lane16);
     };
     auto load_s = [&](int id) {
         const float * p = a.c.scales + ((int64_t) (id < 0 ? 0 : id) * a.c.Hkv + g) * 2;
@@ -418,34 +431,61 @@ __global__ __launch_bounds__(KT) void k_kv8_step(Kv8AttnArgs a) {
     // the rows' bytes
     const uint32_t b = 3 - part, flip = part ? 0x80808080u : 0u;
     const uint32_t sel01 = 0x0c0c0000u | (4 + b) << 8 | b, sel23 = 0x00000c0cu | (4 + b) << 24 | b << 16;
-    auto cut = [&](uint32_t y0, uint32_t y1, uint32_t y2, uint32_t y3) {           // byte `part` of four fixed-point numbers
-        constexpr uint32_t bias = 0x00808080u;
-        return (__builtin_amdgcn_perm(y1 + bias, y0 + bias, sel01) | __builtin_amdgcn_perm(y3 + bias, y2 + bias, sel23)) ^ flip;
+    constexpr int bias = 0x00808080;          // makes the lower three bytes' signed digits unsigned
+    auto cut = [&](uint32_t y0, uint32_t y1, uint32_t y2, uint32_t y3) {           // byte `part` of four biased fixed-point numbers
+        return (__builtin_amdgcn_perm(y1, y0, sel01) | __builtin_amdgcn_perm(y3, y2, sel23)) ^ flip;
     };
-    i32x4 qa[RS][KS];
-    float rowf[RS];
-#pragma unroll
-    for (int k = 0; k < RS; k++) {
+    auto cut_row = [&](int64_t base, i32x4 (&y)[KS]) {           // the bytes of a lane's row, and what a unit of them is worth
+        float q[KS][16];
         uint32_t mq = 0;
 #pragma unroll
-        for (int s = 0; s < KS; s++)
+        for (int s = 0; s < KS; s++) {
+            const int d = 64 * s + 16 * quad;
+            if (a.f32) load16<true>(a.q, base + (d < D ? d : 0), q[s]);
+            else load16<false>(a.q, base + (d < D ? d : 0), q[s]);
 #pragma unroll
-            for (int e = 0; e < 16; e++) mq = max(mq, __float_as_uint(q[k][s][e]) & 0x7fffffffu);
-        float big = __uint_as_float(mq);                         // NaN (as a number the largest) has to win
+            for (int e = 0; e < 16; e++) {
+                if (d >= D) q[s][e] = 0.f;
+                mq = max(mq, __float_as_uint(q[s][e]) & 0x7fffffffu);            // (a NaN is the largest)
+            }
+        }
         mq = max(mq, (uint32_t) __shfl_xor((int) mq, 16));
         mq = max(mq, (uint32_t) __shfl_xor((int) mq, 32));
-        big = __uint_as_float(mq);
-        const int e2 = mq >= 0x7f800000u ? 0 : __builtin_amdgcn_frexp_expf(big);     // big < 2^e2
-        rowf[k] = mq >= 0x7f800000u ? nan : ldexpf(MASK ? a.scale : a.scale * LOG2E, e2 - 30);
+        const int e2 = mq >= 0x7f800000u ? 0 : __builtin_amdgcn_frexp_expf(__uint_as_float(mq));     // the largest < 2^e2
 #pragma unroll
         for (int s = 0; s < KS; s++)
 #pragma unroll
             for (int u = 0; u < 4; u++) {
-                uint32_t y[4];
+                uint32_t x[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) y[e] = (uint32_t) (int) rintf(ldexpf(q[k][s][4 * u + e], 30 - e2));
-                qa[k][s][u] = cut(y[0], y[1], y[2], y[3]);
+                for (int e = 0; e < 4; e++) x[e] = (uint32_t) (int) rintf(ldexpf(q[s][4 * u + e], 30 - e2)) + bias;
+                y[s][u] = cut(x[0], x[1], x[2], x[3]);
             }
+        return mq >= 0x7f800000u ? nan : ldexpf(MASK ? a.scale : a.scale * LOG2E, e2 - 30);
+    };
+    i32x4 qa[RS][KS];
+    float rowf[RS];
+    if (RS == 1) {
+        rowf[0] = cut_row(qat[0], qa[0]);
+    } else {                                                     // a set a wave, shared through LDS
+        i32x4 * fq = (i32x4 *) (lds + SW * HG * (D + 2));
+        float * ff = (float *) (fq + RS * KS * 64);
+        if (w < RS) {
+            int64_t at = qat[0];
+#pragma unroll
+            for (int k = 1; k < RS; k++) at = w == k ? qat[k] : at;
+            i32x4 y[KS];
+            ff[w * 64 + lane] = cut_row(at, y);
+#pragma unroll
+            for (int s = 0; s < KS; s++) fq[(w * KS + s) * 64 + lane] = y[s];
+        }
+        lds_barrier();
+#pragma unroll
+        for (int k = 0; k < RS; k++) {
+            rowf[k] = ff[k * 64 + lane];
+#pragma unroll
+            for (int s = 0; s < KS; s++) qa[k][s] = fq[(k * KS + s) * 64 + lane];
+        }
     }
     const float pw = __uint_as_float((127u + 8 * b) << 23);      // 256^(3 - part)
     float m[RS], l[RS], acc[RS][NC];
@@ -459,44 +499,36 @@ __global__ __launch_bounds__(KT) void k_kv8_step(Kv8AttnArgs a) {
     for (; pg < pend; pg += SW) {
         const int t0 = pg * KV8_PAGE, next = pg + SW < pend ? kv8_page(tab, pg + SW, a.t.P, a.c.pages) : -1;
         const float skc = sk, svc = sv;
-        i32x4 sc[RS][4];
+        f32x4 mk[4];
+        if (MASK)                             // (ahead of the next page's loads, which would be waited for with it)
 #pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int k = 0; k < RS; k++) {
-                i32x4 d = {0, 0, 0, 0};
-#pragma unroll
-                for (int s = 0; s < KS; s++)
-                    d = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, kr[t][s]), qa[k][s], d, 0, 0, 0);
-                sc[k][t] = d;
-            }
-        if (pg + SW < pend) { load_k(next); load_s(next); }
-        float4 mk[4];
-        if (MASK) {
-            const __amdgpu_buffer_rsrc_t mr = __builtin_amdgcn_make_buffer_rsrc(
-                (void *) (a.mask + i * a.mld + t0), (short) 0, 4 * (hi - t0 < KV8_PAGE ? hi - t0 : KV8_PAGE), 0x00020000);
-#pragma unroll
-            for (int t = 0; t < 4; t++) {
-                mk[t].x = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(mr, 4 * (16 * t + 4 * quad), 0, 0));
-                mk[t].y = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(mr, 4 * (16 * t + 4 * quad) + 4, 0, 0));
-                mk[t].z = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(mr, 4 * (16 * t + 4 * quad) + 8, 0, 0));
-                mk[t].w = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(mr, 4 * (16 * t + 4 * quad) + 12, 0, 0));
-            }
-        }
+            for (int t = 0; t < 4; t++) mk[t] = mask4(a.mask + i * a.mld + t0, 16 * t + 4 * quad, hi - t0);
         const bool edge = t0 < last.lo || t0 + KV8_PAGE > first.hi || t0 < lo || t0 + KV8_PAGE > hi;
         i32x4 pa[RS];
         float al[RS];
         bool up = false;
 #pragma unroll
         for (int k = 0; k < RS; k++) {
-            const float f = rowf[k] * skc;
+            if (RS * NC > 16) __builtin_amdgcn_sched_barrier(0);             // (a set at a time, or its registers are not enough)
+            const float f = rowf[k] * skc * pw;              // of this lane's byte
             float x[16];
+            i32x4 sc[4];
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                sc[t] = (i32x4){0, 0, 0, 0};
+#pragma unroll
+                for (int s = 0; s < KS; s++)
+                    sc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, kr[t][s]), qa[k][s], sc[t], 0, 0, 0);
+            }
+            if (k == RS - 1 && pg + SW < pend) { load_k(next); load_s(next); }
 #pragma unroll
             for (int t = 0; t < 4; t++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    float y = quad_sum((float) sc[k][t][e] * pw) * f;
-                    if (MASK) y += e == 0 ? mk[t].x : (e == 1 ? mk[t].y : (e == 2 ? mk[t].z : mk[t].w));
+                    float y = (float) sc[t][e] * f;
+                    asm("" : "+v"(y));        // (fused with the sum's first addition, the four lanes would round apart, and
+                    y = quad_sum(y);          // the bytes that each cuts from its weight would not belong together)
+                    if (MASK) y += mk[t][e];
                     x[4 * t + e] = y;
                 }
             if (edge) {
@@ -523,7 +555,7 @@ __global__ __launch_bounds__(KT) void k_kv8_step(Kv8AttnArgs a) {
                 for (int e = 0; e < 4; e++) {
                     const float p = __builtin_amdgcn_exp2f(MASK ? (x[4 * t + e] - base) * LOG2E : x[4 * t + e] - base);
                     sum += p;
-                    y[e] = (uint32_t) (int) fmaf(p, 1073741824.f, 0.5f);
+                    y[e] = (uint32_t) (int) fmaf(p, 1073741824.f, (float) bias);        // (past 2^23: rounded to a whole number)
                 }
                 pa[k][t] = cut(y[0], y[1], y[2], y[3]);
             }
@@ -545,13 +577,15 @@ __global__ __launch_bounds__(KT) void k_kv8_step(Kv8AttnArgs a) {
             if (svc != svc && !__shfl((int) (rlo[k] < t0 + KV8_PAGE && rhi[k] > t0), 4 * quad)) fh[k] = fl[k] = 0.f;
         }                                                        // (NaN only where a row sees the page)
 #pragma unroll
-        for (int n = 0; n < NC; n++)
+        for (int n = 0; n < NC; n++) {
+            if (n * RS % 4 == 0) __builtin_amdgcn_sched_barrier(0);          // (four products' results at a time)
 #pragma unroll
             for (int k = 0; k < RS; k++) {
                 const i32x4 d = __builtin_amdgcn_mfma_i32_16x16x64_i8(pa[k], __builtin_bit_cast(i32x4, vr[n]), (i32x4){0, 0, 0, 0}, 0, 0, 0);
                 acc[k][n] = fmaf((float) ((d[0] << 8) + d[1]), fh[k], acc[k][n]);
                 acc[k][n] = fmaf((float) ((d[2] << 8) + d[3]), fl[k], acc[k][n]);
             }
+        }
         if (pg + SW < pend) load_v(next);
     }
     // the waves' rows meet
@@ -570,7 +604,7 @@ __global__ __launch_bounds__(KT) void k_kv8_step(Kv8AttnArgs a) {
     __syncthreads();
     const float unit = MASK ? LOG2E : 1.f;                       // (maxima are in powers of 2 without a mask)
     float * wml = a.ws + a.t.T * a.Hq * a.nch * D;
-    for (int u = threadIdx.x; u < nrow * D; u += KT) {
+    for (int u = threadIdx.x; u < nrow * D; u += 64 * SW) {
         const int rr = u / D, d = u - rr * D;
         const int R = R0 + rr, j = R / a.rep, h = g * a.rep + (R - j * a.rep);
         const int64_t o = (r.row + j) * a.Hq + h;
@@ -623,13 +657,6 @@ __device__ __forceinline__ void codes_f16(uint32_t u, uint32_t & lo, uint32_t & 
     hi = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + k);
 }
 
-// a workgroup barrier that orders LDS accesses only: global loads stay in flight across it
-__device__ __forceinline__ void lds_barrier() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-    __builtin_amdgcn_s_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-}
-
 template <int NC, int WV, int KS, bool MASK>
 __global__ __launch_bounds__(64 * WV, NC <= 8 ? 8 / WV : 1) void k_kv8_tile(Kv8AttnArgs a) {
     constexpr int WR = WV / KS, TR = 32 * WR, NU = 2 * NC / WR, ND = NC / 2;         // waves over the rows, rows, a wave's load
@@ -662,7 +689,8 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 ? 8 / WV : 1) void k_kv8_tile(Kv8A
     const float nan = __uint_as_float(0x7fc00000u), inf = __builtin_inff();
 
     // this wave's share of a page: where each unit's 16 bytes are, and the fragments that they make
-    int src[NU], dst[NU][2];
+    uint32_t src[NU];
+    int dst[NU][2];
 #pragma unroll
     for (int u = 0; u < NU; u++) {
         const int k = w + WR * u;
@@ -776,6 +804,13 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 ? 8 / WV : 1) void k_kv8_tile(Kv8A
         lds_barrier();                                           // cur is whole, the other buffer is read
         const bool skip = !live || n >= np || t0 >= wlast.hi || t0 + KV8_PAGE <= wfirst.lo;
         f32x16 sc[2];
+        f32x4 mk[2][4];
+        if (MASK && !skip) {                  // (ahead of the next page's loads, which would be waited for with it)
+#pragma unroll
+            for (int T = 0; T < 2; T++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) mk[T][e] = mask4(a.mask + i * a.mld + t0, 32 * T + 8 * e + 4 * half, hi - t0);
+        }
         if (!skip) {
             // fragments four products ahead of their use, held in this order (the scheduler would read each just before it)
             uint4 fr[4];
@@ -807,14 +842,10 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 ? 8 / WV : 1) void k_kv8_tile(Kv8A
         const float cs0 = rowf * skc, cs = cs0 < 1e-35f ? 1e-35f : cs0;      // (above 0, so that -inf stays -inf; a NaN stays)
         const bool edge = t0 < wlast.lo || t0 + KV8_PAGE > wfirst.hi || t0 < lo || t0 + KV8_PAGE > hi;
         if (MASK) {
-            const __amdgpu_buffer_rsrc_t mr = __builtin_amdgcn_make_buffer_rsrc(
-                (void *) (a.mask + i * a.mld + t0), (short) 0, 4 * (hi - t0 < KV8_PAGE ? hi - t0 : KV8_PAGE), 0x00020000);
 #pragma unroll
             for (int T = 0; T < 2; T++)
 #pragma unroll
-                for (int e = 0; e < 16; e++)
-                    sc[T][e] = fmaf(sc[T][e], cs, __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
-                                                      mr, 4 * (32 * T + 8 * (e >> 2) + 4 * half + (e & 3)), 0, 0)));
+                for (int e = 0; e < 16; e++) sc[T][e] = fmaf(sc[T][e], cs, mk[T][e >> 2][e & 3]);
         }
         if (edge) {
             const int l0 = (mine.lo > lo ? mine.lo : lo) - t0 - 4 * half, h0 = (mine.hi < hi ? mine.hi : hi) - t0 - 4 * half;
@@ -975,13 +1006,14 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 ? 8 / WV : 1) void k_kv8_tile(Kv8A
 // rows of few.
 template <int W>
 __global__ __launch_bounds__(KT) void k_kv8_combine(Kv8AttnArgs a) {
-    __shared__ float sw[SW][64];
-    __shared__ f32x4 sred[SW][64];
+    constexpr int CW = KT / 64;
+    __shared__ float sw[CW][64];
+    __shared__ f32x4 sred[CW][64];
     const int D = a.c.D, i = blockIdx.y, lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int rh = blockIdx.x * (SW / W) + w / W, h = rh % a.Hq, j = rh / a.Hq, part = w % W;
+    const int rh = blockIdx.x * (CW / W) + w / W, h = rh % a.Hq, j = rh / a.Hq, part = w % W;
     const Kv8Rows r = kv8_rows(a.t.off, i, a.t.T, a.t.max_n);
     const bool live = j < r.n;
-    if (W == 1 ? !live : (blockIdx.x * (SW / W)) / a.Hq >= r.n) return;       // (W > 1 meets at a barrier: leave together)
+    if (W == 1 ? !live : (blockIdx.x * (CW / W)) / a.Hq >= r.n) return;       // (W > 1 meets at a barrier: leave together)
     const int full = a.t.pos[i] < 0 ? 0 : a.t.pos[i], len = full < a.max_len ? full : a.max_len;
     const Kv8Seen s = kv8_seen((int64_t) full - r.n + j, len, a.window);
     const int ca = s.lo / a.C, cb = live && s.hi > s.lo ? (s.hi - 1) / a.C + 1 : ca;         // the chunks that this row sees
@@ -1027,13 +1059,13 @@ __global__ __launch_bounds__(KT) void k_kv8_combine(Kv8AttnArgs a) {
 }
 
 // tile: k_kv8_tile's plan, else k_kv8_step's
-struct AttnPlan { bool tile; int RS, ngrp, C, nch, fold, wv, ks; };
+struct AttnPlan { bool tile; int RS, ngrp, C, nch, fold, wv, ks, sw; };
 
 AttnPlan attn_plan(int f32, int Hq, int D, int Hkv, int nseq, int max_n, int max_len, int window) {
     AttnPlan p;
     const int64_t rows = (int64_t) max_n * (Hq / Hkv);
     p.tile = !f32 && rows > 16;
-    p.RS = rows <= 4 ? 1 : (rows <= 8 ? 2 : 4);
+    p.RS = rows <= 4 ? 1 : (rows <= 8 || D > 64 ? 2 : 4);        // (four sets' registers fit beside the codes of D = 64)
     p.wv = D <= 64 || (D > 96 && D <= 128) ? 8 : 4;
     p.ks = p.wv == 8 ? 2 : 1;
     if (getenv("X_WV") && D <= 128) p.wv = atoi(getenv("X_WV"));
@@ -1041,15 +1073,24 @@ AttnPlan attn_plan(int f32, int Hq, int D, int Hkv, int nseq, int max_n, int max
     if (p.wv == 4) p.ks = 1;
     const int group = p.tile ? 32 * p.wv / p.ks : 4 * p.RS;
     p.ngrp = (int) ((rows + group - 1) / group);
-    const int64_t wgs = (int64_t) Hkv * p.ngrp * nseq, round = p.tile ? KV8_PAGE : SW * KV8_PAGE;
-    // step: chunks of whole rounds of the waves; tile: enough workgroups for two a CU, chunks of 512 tokens or more
-    int64_t nch = p.tile ? 1 : (1024 + wgs - 1) / wgs, most = (max_len + (p.tile ? 511 : round - 1)) / (p.tile ? 512 : round);
-    const int slots = 256 * 8 / p.wv;
-    if (p.tile && wgs < slots) nch = slots / wgs;
-    if (p.tile && getenv("X_NCH")) nch = atoi(getenv("X_NCH"));
-    if (nch > most) nch = most;
-    int64_t C = (max_len + nch - 1) / nch;
-    C = (C + round - 1) / round * round;
+    const int64_t wgs = (int64_t) Hkv * p.ngrp * nseq, eff = window > 0 && window + max_n < max_len ? window + max_n : max_len;
+    int64_t C;
+    if (p.tile) {
+        const int64_t slots = 256 * 8 / p.wv;
+        int64_t nch = wgs < slots ? slots / wgs : 1, most = (max_len + 511) / 512;
+        if (getenv("X_NCH")) nch = atoi(getenv("X_NCH"));
+        nch = nch > most ? most : nch;
+        C = ((max_len + nch - 1) / nch + KV8_PAGE - 1) / KV8_PAGE * KV8_PAGE;
+    } else {
+        const int64_t single = 2048;
+        C = eff <= single ? max_len : std::min<int64_t>(std::max<int64_t>(eff * wgs / 512, 512), 2048);
+        if (getenv("X_C")) C = atoi(getenv("X_C"));
+        // eight waves a workgroup where the workgroups leave CUs without
+        p.sw = wgs * ((max_len + C - 1) / C) <= 256 && D <= 128 ? 8 : 4;
+        if (getenv("X_SW") && D <= 128) p.sw = atoi(getenv("X_SW"));
+        const int64_t round = p.sw * KV8_PAGE;
+        C = (C + round - 1) / round * round;
+    }
     p.C = (int) (C > (1 << 30) ? 1 << 30 : C);
     p.nch = (int) ((max_len + (int64_t) p.C - 1) / p.C);
     p.fold = wgs * p.nch <= 512;
@@ -1057,16 +1098,22 @@ AttnPlan attn_plan(int f32, int Hq, int D, int Hkv, int nseq, int max_n, int max
     return p;
 }
 
-template <int NC, int RS> hipError_t run_step(const Kv8AttnArgs & a, const AttnPlan & p, hipStream_t s) {
+template <int NC, int RS, int SW> hipError_t run_step(const Kv8AttnArgs & a, const AttnPlan & p, hipStream_t s) {
     const dim3 grid((unsigned) (a.c.Hkv * p.ngrp), (unsigned) p.nch, (unsigned) a.t.nseq);
-    const size_t lds = sizeof(float) * SW * 4 * RS * (a.c.D + 2);
-    if (a.mask) k_kv8_step<NC, RS, true><<<grid, KT, lds, s>>>(a);
-    else k_kv8_step<NC, RS, false><<<grid, KT, lds, s>>>(a);
+    const size_t lds = sizeof(float) * SW * 4 * RS * (a.c.D + 2) + (RS > 1 ? RS * ((NC + 3) / 4 * 1024 + 256) : 0);
+    if (a.mask) k_kv8_step<NC, RS, SW, true><<<grid, 64 * SW, lds, s>>>(a);
+    else k_kv8_step<NC, RS, SW, false><<<grid, 64 * SW, lds, s>>>(a);
     return hipGetLastError();
 }
 
 template <int NC> hipError_t run_attn(const Kv8AttnArgs & a, const AttnPlan & p, hipStream_t s) {
-    if (!p.tile) return p.RS == 1 ? run_step<NC, 1>(a, p, s) : (p.RS == 2 ? run_step<NC, 2>(a, p, s) : run_step<NC, 4>(a, p, s));
+    if (!p.tile) {
+        if constexpr (NC <= 4)
+            if (p.RS == 4) return p.sw == 8 ? run_step<NC, 4, 8>(a, p, s) : run_step<NC, 4, 4>(a, p, s);
+        if constexpr (NC <= 8)
+            if (p.sw == 8) return p.RS == 1 ? run_step<NC, 1, 8>(a, p, s) : run_step<NC, 2, 8>(a, p, s);
+        return p.RS == 1 ? run_step<NC, 1, 4>(a, p, s) : run_step<NC, 2, 4>(a, p, s);
+    }
     const dim3 grid((unsigned) (a.c.Hkv * p.ngrp), (unsigned) p.nch, (unsigned) a.t.nseq);
     const size_t lds = 2 * 4 * NC * 1024;
     if constexpr (NC <= 8 && NC % 4 == 0)
@@ -1127,6 +1174,6 @@ hipError_t launch_kv8_attn(const Kv8Cache & c, const Kv8Table & t, const void * 
     if (e != hipSuccess || p.nch == 1) return e;
     const int64_t rh = (int64_t) Hq * t.max_n;
     if (p.nch > 16) k_kv8_combine<4><<<dim3((unsigned) rh, (unsigned) t.nseq), KT, 0, s>>>(a);
-    else k_kv8_combine<1><<<dim3((unsigned) ((rh + SW - 1) / SW), (unsigned) t.nseq), KT, 0, s>>>(a);
+    else k_kv8_combine<1><<<dim3((unsigned) ((rh + KT / 64 - 1) / (KT / 64)), (unsigned) t.nseq), KT, 0, s>>>(a);
     return hipGetLastError();
 }
