@@ -339,6 +339,11 @@ __device__ __forceinline__ f32x4 mask4(const float * page, int at, int have) {
     return v;
 }
 
+template <bool NT> __device__ __forceinline__ uint4 load_code(const int8_t * p) {
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+    return NT ? __builtin_bit_cast(uint4, __builtin_nontemporal_load((const u4 *) p)) : *(const uint4 *) p;
+}
+
 // the larger (or the sum) of x and the lane 32, then 16 away
 template <bool MAX> __device__ __forceinline__ float across_quads(float x) {
     typedef unsigned u2 __attribute__((ext_vector_type(2)));
@@ -362,7 +367,7 @@ __device__ __forceinline__ float quad_sum(float x) {
 // product's operand without a move across lanes. A wave takes every fourth page, K of its next one loading
 // once this one's scores are out, V after its products; waves meet in LDS, chunks in k_kv8_combine.
 // RS sets of 4 rows; NC: chunks of 16 d (D / 16 or more).
-template <int NC, int RS, int SW, bool MASK>
+template <int NC, int RS, int SW, bool MASK, bool NT>
 __global__ __launch_bounds__(64 * SW, SW == 8 ? 2 : (RS == 1 ? (NC <= 4 ? 4 : (NC <= 8 ? 3 : (NC <= 12 ? 2 : 1))) : (RS * NC <= 16 ? 2 : 1))) void k_kv8_step(Kv8AttnArgs a) {
     constexpr int KS = (NC + 3) / 4, HG = 4 * RS;
     extern __shared__ __align__(16) float lds[];                 // red [SW][HG][D], ml [SW][HG][2], the rows' bytes for RS > 1
@@ -408,12 +413,12 @@ __global__ __launch_bounds__(64 * SW, SW == 8 ? 2 : (RS == 1 ? (NC <= 4 ? 4 : (N
 #pragma unroll
         for (int t = 0; t < 4; t++)
 #pragma unroll
-            for (int s = 0; s < KS; s++) kr[t][s] = *(const uint4 *) (p + t * nc * 256 + s * 1024 + lane16);
+            for (int s = 0; s < KS; s++) kr[t][s] = load_code<NT>(p + t * nc * 256 + s * 1024 + lane16);
     };
     auto load_v = [&](int id) {               // (chunks past D re-read the last: not stored)
         const int8_t * p = page_base(id) + KV8_PAGE * D;
 #pragma unroll
-        for (int n = 0; n < NC; n++) vr[n] = *(const uint4 *) (p + (n < nc ? n : nc - 1) * 1024 + lane16);
+        for (int n = 0; n < NC; n++) vr[n] = load_code<NT>(p + (n < nc ? n : nc - 1) * 1024 + lane16);
     };
     auto load_s = [&](int id) {
         const float * p = a.c.scales + ((int64_t) (id < 0 ? 0 : id) * a.c.Hkv + g) * 2;
@@ -1059,7 +1064,7 @@ __global__ __launch_bounds__(KT) void k_kv8_combine(Kv8AttnArgs a) {
 }
 
 // tile: k_kv8_tile's plan, else k_kv8_step's
-struct AttnPlan { bool tile; int RS, ngrp, C, nch, fold, wv, ks, sw; };
+struct AttnPlan { bool tile; int RS, ngrp, C, nch, fold, wv, ks, sw; bool nt; };
 
 AttnPlan attn_plan(int f32, int Hq, int D, int Hkv, int nseq, int max_n, int max_len, int window) {
     AttnPlan p;
@@ -1088,6 +1093,9 @@ AttnPlan attn_plan(int f32, int Hq, int D, int Hkv, int nseq, int max_n, int max
         // eight waves a workgroup where the workgroups leave CUs without
         p.sw = wgs * ((max_len + C - 1) / C) <= 256 && D <= 128 ? 8 : 4;
         if (getenv("X_SW") && D <= 128) p.sw = atoi(getenv("X_SW"));
+        // non-temporal loads where the codes are more than the caches would keep for another call (MB, us without -> with: 1070
+        // 187 -> 170, 578 116 -> 103, 245 64 -> 57, 134 27.4 -> 24.1, 67 15.3 -> 15.4, 33 13.6 -> 15.8, 4 11.0 -> 13.6)
+        p.nt = p.ngrp == 1 && 2 * eff * nseq * Hkv * D >= 100000000;
         const int64_t round = p.sw * KV8_PAGE;
         C = (C + round - 1) / round * round;
     }
@@ -1101,8 +1109,9 @@ AttnPlan attn_plan(int f32, int Hq, int D, int Hkv, int nseq, int max_n, int max
 template <int NC, int RS, int SW> hipError_t run_step(const Kv8AttnArgs & a, const AttnPlan & p, hipStream_t s) {
     const dim3 grid((unsigned) (a.c.Hkv * p.ngrp), (unsigned) p.nch, (unsigned) a.t.nseq);
     const size_t lds = sizeof(float) * SW * 4 * RS * (a.c.D + 2) + (RS > 1 ? RS * ((NC + 3) / 4 * 1024 + 256) : 0);
-    if (a.mask) k_kv8_step<NC, RS, SW, true><<<grid, 64 * SW, lds, s>>>(a);
-    else k_kv8_step<NC, RS, SW, false><<<grid, 64 * SW, lds, s>>>(a);
+    if (a.mask) k_kv8_step<NC, RS, SW, true, false><<<grid, 64 * SW, lds, s>>>(a);
+    else if (SW == 4 && RS <= 2 && p.nt) k_kv8_step<NC, RS, SW, false, SW == 4 && RS <= 2><<<grid, 64 * SW, lds, s>>>(a);
+    else k_kv8_step<NC, RS, SW, false, false><<<grid, 64 * SW, lds, s>>>(a);
     return hipGetLastError();
 }
 
