@@ -1968,7 +1968,8 @@ int onpu_kv8_read_dev(const void * codes, const float * scales, int64_t pages, i
 }
 
 int64_t onpu_kv8_attn_ws_bytes(int q_bf16, int Hq, int D, int Hkv, int nseq, int64_t T, int max_n, int max_len, int window) {
-    if (Hq <= 0 || D <= 0 || Hkv <= 0 || Hq % Hkv || nseq <= 0 || T <= 0 || max_n <= 0 || max_len <= 0) return 0;
+    if (Hq <= 0 || D <= 0 || Hkv <= 0 || Hq % Hkv || nseq <= 0 || T <= 0 || max_n <= 0 || max_len <= 0 || max_len > INT32_MAX - 64)
+        return 0;
     return kv8_attn_ws_bytes(!q_bf16, Hq, D, Hkv, nseq, T, max_n, max_len, window);
 }
 
@@ -1980,8 +1981,8 @@ int onpu_kv8_attn_dev(const void * q, int q_bf16, int Hq, int64_t qrs, int64_t q
     Kv8Table t;
     if (!kv8_fill("onpu_kv8_attn_dev", codes, scales, pages, Hkv, D, table, tld, P, lens, off, nseq, T, max_n, c, t)) return -1;
     if (T == 0) return 0;
-    if (Hq <= 0 || Hq % Hkv || max_len < 1 || window < 0 || (mask && mld < max_len)) {
-        set_err("onpu_kv8_attn_dev: needs Hq a multiple of Hkv, max_len >= 1, window >= 0, mask rows of max_len or more");
+    if (Hq <= 0 || Hq % Hkv || max_len < 1 || max_len > INT32_MAX - 64 || window < 0 || (mask && mld < max_len)) {
+        set_err("onpu_kv8_attn_dev: needs Hq a multiple of Hkv, max_len from 1 to 2^31 - 65, window >= 0, mask rows of max_len or more");
         return -1;
     }
     if (T == 1) qrs = 0;

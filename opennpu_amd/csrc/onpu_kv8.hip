@@ -1,7 +1,6 @@
 // The 8-bit key-value cache: quantising tokens into its pages, reading them back, and attention over
 // them. Layout and index arithmetic: onpu_kv8.h.
 #include <algorithm>
-#include <cstdlib>
 
 #include "onpu_launch.h"
 
@@ -62,6 +61,29 @@ __device__ __forceinline__ int quant(float x, float s, float inv) {
     if (e < -h || (e == -h && odd)) c -= 1.f;
     return (int) fminf(fmaxf(c, -127.f), 127.f);
 }
+// the codes of four values, their lowest bytes: x / s + 1.5 2^23 in one fma is the nearest integer (ties to even) of
+// x * (1 / s) in the sum's last bits, right unless the remainder x - c s is within 2^-16 s of s / 2, which `far` (the
+// largest |x - c s| so far) tells: then quant decides
+__device__ __forceinline__ uint32_t near4(const float (&x)[4], float s, float inv, float & far) {
+    uint32_t y[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const float c = fmaf(x[e], inv, 12582912.f);
+        far = fmaxf(far, fabsf(fmaf(-(c - 12582912.f), s, x[e])));
+        y[e] = __float_as_uint(c);
+    }
+    return __builtin_amdgcn_perm(y[1], y[0], 0x0c0c0400u) | __builtin_amdgcn_perm(y[3], y[2], 0x04000c0cu);
+}
+// the largest |value| of raw words, as bits (NaN the largest)
+template <bool F32> __device__ __forceinline__ uint32_t raw_max(uint32_t m, uint4 u) {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        m = F32 ? max(m, w[e] & 0x7fffffffu)
+                : __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, m), __builtin_bit_cast(u16x2, w[e] & 0x7fff7fffu)));
+    return m;
+}
 __device__ __forceinline__ uint32_t bytes4(int a, int b, int c, int d) {
     return (uint32_t) (a & 255) | (uint32_t) (b & 255) << 8 | (uint32_t) (c & 255) << 16 | (uint32_t) d << 24;
 }
@@ -116,11 +138,16 @@ __global__ __launch_bounds__(KT) void k_kv8_write(WriteArgs a) {
 #pragma unroll
         for (int k = 0; k < NK; k++)          // (slots outside repeat slot s0: the maximum is of the new values)
 #pragma unroll
-            for (int e = 0; e < 16; e++) m[0] = max(m[0], __float_as_uint(raw_at<F32>(xk[k], e)) & 0x7fffffffu);
+            for (size_t e = 0; e < sizeof(xk[0]) / 16; e++) m[0] = raw_max<F32>(m[0], xk[k].u[e]);
 #pragma unroll
         for (int k = 0; k < NV; k++)
 #pragma unroll
-            for (int e = 0; e < 32; e++) m[1] = max(m[1], __float_as_uint(raw_at<F32>(xv[k][e >> 3], e & 7)) & 0x7fffffffu);
+            for (int n = 0; n < 4; n++)
+#pragma unroll
+                for (size_t e = 0; e < sizeof(xv[0][0]) / 16; e++) m[1] = raw_max<F32>(m[1], xv[k][n].u[e]);
+        if (!F32)                             // (two bf16 maxima a word)
+#pragma unroll
+            for (int kv = 0; kv < 2; kv++) m[kv] = max(m[kv] << 16, m[kv] & 0xffff0000u);
     }
 #pragma unroll
     for (int kv = 0; kv < 2; kv++) {
@@ -152,6 +179,7 @@ __global__ __launch_bounds__(KT) void k_kv8_write(WriteArgs a) {
     }
     if (s0 > 0) __syncthreads();              // the new bytes go on top (and so has been read by all)
     if (t < 2) sc[t] = t ? s[1] : s[0];
+    const float lim[2] = {s[0] * 0.4999847f, s[1] * 0.4999847f};
     if (some && s0 > 0) {
         for (int kv = 0; kv < 2; kv++)
             for (int u = t; u < (s1 - s0) * D; u += KT) {
@@ -191,12 +219,18 @@ __global__ __launch_bounds__(KT) void k_kv8_write(WriteArgs a) {
         const int u = t + KT * k, tok = u / NC, d = u % NC * 16;
         if (tok >= KV8_PAGE || tok < s0 || (s0 > 0 && tok >= s1)) continue;
         uint32_t y[4];
+        float far = 0.f;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            y[e] = bytes4(quant(raw_at<F32>(xk[k], 4 * e), s[0], inv[0]), quant(raw_at<F32>(xk[k], 4 * e + 1), s[0], inv[0]),
-                          quant(raw_at<F32>(xk[k], 4 * e + 2), s[0], inv[0]), quant(raw_at<F32>(xk[k], 4 * e + 3), s[0], inv[0]));
-            if (tok >= s1) y[e] = 0;
+            const float x[4] = {raw_at<F32>(xk[k], 4 * e), raw_at<F32>(xk[k], 4 * e + 1), raw_at<F32>(xk[k], 4 * e + 2), raw_at<F32>(xk[k], 4 * e + 3)};
+            y[e] = near4(x, s[0], inv[0], far);
         }
+        if (far > lim[0])
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                y[e] = bytes4(quant(raw_at<F32>(xk[k], 4 * e), s[0], inv[0]), quant(raw_at<F32>(xk[k], 4 * e + 1), s[0], inv[0]),
+                              quant(raw_at<F32>(xk[k], 4 * e + 2), s[0], inv[0]), quant(raw_at<F32>(xk[k], 4 * e + 3), s[0], inv[0]));
+        if (tok >= s1) y[0] = y[1] = y[2] = y[3] = 0;
         *(uint4 *) (out + kv8_k_at(D, tok, d)) = make_uint4(y[0], y[1], y[2], y[3]);
     }
     const bool merge = s0 > 0;                // V's words of the page as they are below the new bytes
@@ -210,13 +244,23 @@ __global__ __launch_bounds__(KT) void k_kv8_write(WriteArgs a) {
         for (int e = 0; e < 4; e++)
             if (4 * q + e < s0 || 4 * q + e >= s1) keep |= 255u << (8 * e);
         if (merge && keep == 0xffffffffu) continue;
+        uint32_t y[8];
+        float far = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float x[4] = {raw_at<F32>(xv[k][0], e), raw_at<F32>(xv[k][1], e), raw_at<F32>(xv[k][2], e), raw_at<F32>(xv[k][3], e)};
+            y[e] = near4(x, s[1], inv[1], far);
+        }
+        if (far > lim[1])
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                y[e] = bytes4(quant(raw_at<F32>(xv[k][0], e), s[1], inv[1]), quant(raw_at<F32>(xv[k][1], e), s[1], inv[1]),
+                              quant(raw_at<F32>(xv[k][2], e), s[1], inv[1]), quant(raw_at<F32>(xv[k][3], e), s[1], inv[1]));
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const int at = kv8_v_at(D, 4 * q, d + e);
-            const uint32_t y = bytes4(quant(raw_at<F32>(xv[k][0], e), s[1], inv[1]), quant(raw_at<F32>(xv[k][1], e), s[1], inv[1]),
-                                      quant(raw_at<F32>(xv[k][2], e), s[1], inv[1]), quant(raw_at<F32>(xv[k][3], e), s[1], inv[1]));
-            if (merge) *(uint32_t *) (ov + at) = (y & ~keep) | (keep ? *(uint32_t *) (ov + at) & keep : 0);
-            else vt[at / 4] = y & ~keep;
+            if (merge) *(uint32_t *) (ov + at) = (y[e] & ~keep) | (keep ? *(uint32_t *) (ov + at) & keep : 0);
+            else vt[at / 4] = y[e] & ~keep;
         }
     }
     if (merge) return;
@@ -679,9 +723,7 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 ? 8 / WV : 1) void k_kv8_tile(Kv8A
     if (z >= ngrp) return;
     // the longest first; with no more workgroups than run at once, the second half the shortest first, so that
     // what two workgroups of a CU have adds to the same
-    if (a.fold == 1) z = z >= ngrp / 2 ? z - ngrp / 2 : ngrp - 1 - z;
-    else if (a.fold == 2) z = z & 1 ? z / 2 : ngrp - 1 - z / 2;
-    else if (a.fold == 0) z = ngrp - 1 - z;
+    z = a.fold && z >= ngrp / 2 ? z - ngrp / 2 : ngrp - 1 - z;
     const int R0 = z * TR, nrow = rows - R0 < TR ? rows - R0 : TR;
     const int full = a.t.pos[i] < 0 ? 0 : a.t.pos[i], len = full < a.max_len ? full : a.max_len;
     const int64_t at0 = (int64_t) full - r.n;
@@ -892,9 +934,12 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 ? 8 / WV : 1) void k_kv8_tile(Kv8A
                 eref = e;
             }
 #pragma unroll
-            for (int t = 0; t < ND; t++)
-#pragma unroll
+            for (int t = 0; t < ND; t++) {
+                if (NC > 8) asm volatile("" : "+a"(o[t]));       // (o stays in accumulation registers but here, where it is
+#pragma unroll                                                   //  read and written back; without this each page copied it)
                 for (int e = 0; e < 16; e++) o[t][e] *= f;
+                if (NC > 8) asm volatile("" : "+a"(o[t]));
+            }
         }
         // weights: 2^8 e^(x - m) sv 2^-eref in fp16
         const float base = m == -inf ? 0.f : m, lr = 8.f + (lsc - (float) eref);
@@ -1063,6 +1108,48 @@ __global__ __launch_bounds__(KT) void k_kv8_combine(Kv8AttnArgs a) {
     }
 }
 
+// ... and of few chunks (up to J): D / 4 lanes a row, 4 columns each, every chunk's maximum, sum and columns loaded at
+// once. (512 x 40 rows of 3 chunks: 15.5 us by the kernel above, which goes through LDS and two more latencies.)
+template <int J>
+__global__ __launch_bounds__(KT) void k_kv8_join(Kv8AttnArgs a) {
+    const int D = a.c.D, DL = D / 4, i = blockIdx.y, u = blockIdx.x * KT + threadIdx.x, rh = u / DL, d = (u - rh * DL) * 4;
+    const int h = rh % a.Hq, j = rh / a.Hq;
+    const Kv8Rows r = kv8_rows(a.t.off, i, a.t.T, a.t.max_n);
+    if (j >= r.n) return;
+    const int full = a.t.pos[i] < 0 ? 0 : a.t.pos[i], len = full < a.max_len ? full : a.max_len;
+    const Kv8Seen s = kv8_seen((int64_t) full - r.n + j, len, a.window);
+    const int ca = s.lo / a.C, n = s.hi > s.lo ? (s.hi - 1) / a.C + 1 - ca : 0;         // the chunks that this row sees
+    const int64_t o = (r.row + j) * a.Hq + h;
+    const float * wo = a.ws + (o * a.nch + ca) * D + d, * wml = a.ws + a.t.T * a.Hq * a.nch * D + (o * a.nch + ca) * 2;
+    const float unit = a.mask ? LOG2E : 1.f, sink = a.sinks ? a.sinks[h] * (a.mask ? 1.f : LOG2E) : -__builtin_inff();
+    float mc[J], lc[J];
+    f32x4 x[J];
+#pragma unroll
+    for (int k = 0; k < J; k++) {             // (past the row's chunks its first again, unused; none: nothing is read)
+        const int c = k < n ? k : 0;
+        mc[k] = n > 0 ? wml[2 * c] : -__builtin_inff();
+        lc[k] = n > 0 ? wml[2 * c + 1] : 0.f;
+        x[k] = n > 0 ? *(const f32x4 *) (wo + (int64_t) c * D) : (f32x4){0, 0, 0, 0};
+    }
+    float M = sink, den = 0.f;
+#pragma unroll
+    for (int k = 0; k < J; k++) M = k < n ? fmaxf(M, mc[k]) : M;
+    const float base = M == -__builtin_inff() ? 0.f : M;
+    f32x4 y = {0, 0, 0, 0};
+#pragma unroll
+    for (int k = 0; k < J; k++)
+        if (k < n) {
+            const float f = __builtin_amdgcn_exp2f((mc[k] - base) * unit);
+            den += f * lc[k];
+            y += f * x[k];
+        }
+    if (a.sinks) den += __builtin_amdgcn_exp2f((sink - base) * unit);
+    const float f = 1.f / den;
+    const float4 v = den == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(y[0] * f, y[1] * f, y[2] * f, y[3] * f);
+    if (a.f32) *(float4 *) ((float *) a.out + o * D + d) = v;
+    else *(uint2 *) ((uint16_t *) a.out + o * D + d) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
+}
+
 // tile: k_kv8_tile's plan, else k_kv8_step's
 struct AttnPlan { bool tile; int RS, ngrp, C, nch, fold, wv, ks, sw; bool nt; };
 
@@ -1071,28 +1158,28 @@ AttnPlan attn_plan(int f32, int Hq, int D, int Hkv, int nseq, int max_n, int max
     const int64_t rows = (int64_t) max_n * (Hq / Hkv);
     p.tile = !f32 && rows > 16;
     p.RS = rows <= 4 ? 1 : (rows <= 8 || D > 64 ? 2 : 4);        // (four sets' registers fit beside the codes of D = 64)
-    p.wv = D <= 64 || (D > 96 && D <= 128) ? 8 : 4;
-    p.ks = p.wv == 8 ? 2 : 1;
-    if (getenv("X_WV") && D <= 128) p.wv = atoi(getenv("X_WV"));
-    if (getenv("X_KS")) p.ks = atoi(getenv("X_KS"));
-    if (p.wv == 4) p.ks = 1;
+    // The prompt kernel's workgroups: 8 waves over 256 rows where every row sees nearly the same tokens, 8 waves in two
+    // groups over 128 rows where there are no more, else 4 waves over 128 rows, which balance a causal triangle better.
+    // (8 waves need whole units of a page: D up to 64 and from 97 to 128.)
+    const bool eight = D <= 64 || (D > 96 && D <= 128);
+    p.wv = eight && (rows <= 128 || (int64_t) max_n * 4 <= max_len) ? 8 : 4;
+    p.ks = p.wv == 8 && rows <= 128 ? 2 : 1;
     const int group = p.tile ? 32 * p.wv / p.ks : 4 * p.RS;
     p.ngrp = (int) ((rows + group - 1) / group);
     const int64_t wgs = (int64_t) Hkv * p.ngrp * nseq, eff = window > 0 && window + max_n < max_len ? window + max_n : max_len;
     int64_t C;
     if (p.tile) {
-        const int64_t slots = 256 * 8 / p.wv;
-        int64_t nch = wgs < slots ? slots / wgs : 1, most = (max_len + 511) / 512;
-        if (getenv("X_NCH")) nch = atoi(getenv("X_NCH"));
+        // split along the tokens where the workgroups leave CUs without, in chunks of 512 or more; not for twofold gains,
+        // which the partials and the join cost again
+        const int64_t slots = p.wv == 8 || D > 128 ? 256 : 512;
+        int64_t nch = slots / wgs >= 3 ? slots / wgs : 1, most = (max_len + 511) / 512;
         nch = nch > most ? most : nch;
         C = ((max_len + nch - 1) / nch + KV8_PAGE - 1) / KV8_PAGE * KV8_PAGE;
     } else {
         const int64_t single = 2048;
         C = eff <= single ? max_len : std::min<int64_t>(std::max<int64_t>(eff * wgs / 512, 512), 2048);
-        if (getenv("X_C")) C = atoi(getenv("X_C"));
         // eight waves a workgroup where the workgroups leave CUs without
         p.sw = wgs * ((max_len + C - 1) / C) <= 256 && D <= 128 ? 8 : 4;
-        if (getenv("X_SW") && D <= 128) p.sw = atoi(getenv("X_SW"));
         // non-temporal loads where the codes are more than the caches would keep for another call (MB, us without -> with: 1070
         // 187 -> 170, 578 116 -> 103, 245 64 -> 57, 134 27.4 -> 24.1, 67 15.3 -> 15.4, 33 13.6 -> 15.8, 4 11.0 -> 13.6)
         p.nt = p.ngrp == 1 && 2 * eff * nseq * Hkv * D >= 100000000;
@@ -1101,8 +1188,7 @@ AttnPlan attn_plan(int f32, int Hq, int D, int Hkv, int nseq, int max_n, int max
     }
     p.C = (int) (C > (1 << 30) ? 1 << 30 : C);
     p.nch = (int) ((max_len + (int64_t) p.C - 1) / p.C);
-    p.fold = wgs * p.nch <= 512;
-    if (getenv("X_FOLD")) p.fold = atoi(getenv("X_FOLD"));
+    p.fold = p.wv == 4 && wgs * p.nch <= 512;
     return p;
 }
 
@@ -1175,14 +1261,17 @@ hipError_t launch_kv8_attn(const Kv8Cache & c, const Kv8Table & t, const void * 
                            void * out, void * ws, hipStream_t s) {
     const AttnPlan p = attn_plan(f32, Hq, c.D, c.Hkv, t.nseq, t.max_n, max_len, window);
     Kv8AttnArgs a{c, t, q, out, mask, sinks, (float *) ws, qrs, qhs, mld, scale, Hq, Hq / c.Hkv, max_len, window, f32, p.C, p.nch, p.fold};
-    if (!grid_fits((int64_t) Hq * t.max_n, t.nseq) || !grid_fits((int64_t) c.Hkv * p.ngrp, t.nseq) || p.nch > 65535)
+    if (!grid_fits((int64_t) Hq * t.max_n * (c.D / 4) / KT + 1, t.nseq) || !grid_fits((int64_t) Hq * t.max_n, t.nseq) || !grid_fits((int64_t) c.Hkv * p.ngrp, t.nseq) || p.nch > 65535)
         return hipErrorInvalidValue;
     const int nc = c.D / 16;
     hipError_t e = nc <= 4 ? run_attn<4>(a, p, s) : (nc <= 6 ? run_attn<6>(a, p, s) : (nc <= 8 ? run_attn<8>(a, p, s) :
                    (nc <= 12 ? run_attn<12>(a, p, s) : run_attn<16>(a, p, s))));
     if (e != hipSuccess || p.nch == 1) return e;
     const int64_t rh = (int64_t) Hq * t.max_n;
-    if (p.nch > 16) k_kv8_combine<4><<<dim3((unsigned) rh, (unsigned) t.nseq), KT, 0, s>>>(a);
+    const dim3 join((unsigned) ((rh * (c.D / 4) + KT - 1) / KT), (unsigned) t.nseq);
+    if (p.nch <= 4) k_kv8_join<4><<<join, KT, 0, s>>>(a);
+    else if (p.nch <= 8) k_kv8_join<8><<<join, KT, 0, s>>>(a);
+    else if (p.nch > 16) k_kv8_combine<4><<<dim3((unsigned) rh, (unsigned) t.nseq), KT, 0, s>>>(a);
     else k_kv8_combine<1><<<dim3((unsigned) ((rh + KT / 64 - 1) / (KT / 64)), (unsigned) t.nseq), KT, 0, s>>>(a);
     return hipGetLastError();
 }

@@ -113,7 +113,7 @@ MORE = {
     "write": [dict(k=None), dict(v=None), dict(pos=None), dict(k=(1 << 20) + 8), dict(krs=132), dict(khs=4), dict(vrs=1), dict(vhs=12),
               dict(bf16=0, krs=130), dict(max_n=2 ** 31 - 1)],
     "read": [dict(k=None), dict(v=None), dict(pos=None), dict(v=(1 << 20) + 4), dict(max_n=2 ** 31 - 1)],
-    "attn": [dict(q=None), dict(out=None), dict(lens=None), dict(Hq=3), dict(Hq=0), dict(qrs=4), dict(qhs=2), dict(max_len=0),
+    "attn": [dict(q=None), dict(out=None), dict(lens=None), dict(Hq=3), dict(Hq=0), dict(qrs=4), dict(qhs=2), dict(max_len=0), dict(max_len=2 ** 31 - 64),
              dict(window=-1), dict(mask=1 << 20, mld=99), dict(out=(1 << 20) + 4)],
 }
 
