@@ -706,8 +706,10 @@ __device__ __forceinline__ void codes_f16(uint32_t u, uint32_t & lo, uint32_t & 
     hi = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + k);
 }
 
-template <int NC, int WV, int KS, bool MASK>
-__global__ __launch_bounds__(64 * WV, NC <= 8 ? 8 / WV : 1) void k_kv8_tile(Kv8AttnArgs a) {
+template <int NC, int WV, int KS, bool MASK, bool F32>
+__global__ __launch_bounds__(64 * WV, NC <= 8 && !F32 ? 8 / WV : 1) void k_kv8_tile(Kv8AttnArgs a) {
+    constexpr int PARTS = F32 ? 2 : 1;        // fp16 parts of q and of a weight
+    constexpr bool ACC = NC > 8 || F32;       // more than 256 registers: o stays in accumulation registers
     constexpr int WR = WV / KS, TR = 32 * WR, NU = 2 * NC / WR, ND = NC / 2;         // waves over the rows, rows, a wave's load
     constexpr int FRAGS = 4 * NC;                                                    // units, d tiles of 32, KiB of a page
     static_assert(NU * WR == 2 * NC, "the waves share a page's units evenly");
@@ -801,34 +803,35 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 ? 8 / WV : 1) void k_kv8_tile(Kv8A
     const bool live = w * 32 < nrow;                             // a wave behind the last row only loads
     const int wl = live ? w * 32 : nrow - 1, wh = w * 32 + 31 < nrow ? w * 32 + 31 : nrow - 1;
     const Kv8Seen wfirst = kv8_seen(at0 + (R0 + wl) / a.rep, len, a.window), wlast = kv8_seen(at0 + (R0 + wh) / a.rep, len, a.window);
-    f16x8 q[NC];
+    f16x8 q[PARTS][NC];
     float rowf;
     {
-        const uint16_t * p = (const uint16_t *) a.q + (r.row + j) * a.qrs + h * a.qhs;
-        uint4 u[NC];
+        const int64_t base = (r.row + j) * a.qrs + h * a.qhs;
+        Raw8<F32> u[NC];
         uint32_t mq = 0;
 #pragma unroll
-        for (int s2 = 0; s2 < NC / 2; s2++)
+        for (int k = 0; k < NC; k++) {
+            const int d = 16 * (k / 2 * 2 + half) + 8 * (k & 1);
+            u[k] = load_raw<F32, Raw8<F32>>(a.q, base + (d < D ? d : 0));
 #pragma unroll
-            for (int v = 0; v < 2; v++) {
-                const int d = 16 * (2 * s2 + half) + 8 * v;
-                uint4 x = *(const uint4 *) (p + (d < D ? d : 0));
-                if (d >= D) x = make_uint4(0, 0, 0, 0);
-                u[2 * s2 + v] = x;
-                mq = max(mq, max(max(x.x & 0x7fff0000u, x.y & 0x7fff0000u), max(x.z & 0x7fff0000u, x.w & 0x7fff0000u)));
-                mq = max(mq, max(max(x.x << 16 & 0x7fff0000u, x.y << 16 & 0x7fff0000u), max(x.z << 16 & 0x7fff0000u, x.w << 16 & 0x7fff0000u)));
+            for (size_t e = 0; e < sizeof(u[0]) / 16; e++) {
+                if (d >= D) u[k].u[e] = make_uint4(0, 0, 0, 0);
+                mq = raw_max<F32>(mq, u[k].u[e]);
             }
+        }
+        if (!F32) mq = max(mq << 16, mq & 0xffff0000u);
         mq = max(mq, (uint32_t) __shfl_xor((int) mq, 32));
         const int e2 = mq >= 0x7f800000u ? 0 : __builtin_amdgcn_frexp_expf(__uint_as_float(mq));     // the largest < 2^e2, to 2^8
         rowf = mq >= 0x7f800000u ? nan : ldexpf(fabsf(a.scale) * (MASK ? 1.f : LOG2E), e2 - 8);
         const float sign = a.scale < 0.f ? -1.f : 1.f;
 #pragma unroll
-        for (int k = 0; k < NC; k++) {
-            const uint32_t x[4] = {u[k].x, u[k].y, u[k].z, u[k].w};
+        for (int k = 0; k < NC; k++)
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-                q[k][e] = (_Float16) ldexpf(sign * (e & 1 ? bf_hi(x[e / 2]) : bf_lo(x[e / 2])), 8 - e2);
-        }
+            for (int e = 0; e < 8; e++) {
+                const float x = ldexpf(sign * raw_at<F32>(u[k], e), 8 - e2);
+                q[0][k][e] = (_Float16) x;
+                if (F32) q[PARTS - 1][k][e] = (_Float16) (x - (float) q[0][k][e]);
+            }
     }
     f32x16 o[ND];
 #pragma unroll
@@ -870,7 +873,9 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 ? 8 / WV : 1) void k_kv8_tile(Kv8A
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int k = 0; k < 2 * NC; k++) {
-                sc[k / NC] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, fr[k & 3]), q[k % NC], sc[k / NC], 0, 0, 0);
+#pragma unroll
+                for (int y = 0; y < PARTS; y++)
+                    sc[k / NC] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, fr[k & 3]), q[y][k % NC], sc[k / NC], 0, 0, 0);
                 if (k + 4 < 2 * NC) fr[k & 3] = cur[(k + 4) * 64 + lane];
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -935,10 +940,10 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 ? 8 / WV : 1) void k_kv8_tile(Kv8A
             }
 #pragma unroll
             for (int t = 0; t < ND; t++) {
-                if (NC > 8) asm volatile("" : "+a"(o[t]));       // (o stays in accumulation registers but here, where it is
+                if (ACC) asm volatile("" : "+a"(o[t]));       // (o stays in accumulation registers but here, where it is
 #pragma unroll                                                   //  read and written back; without this each page copied it)
                 for (int e = 0; e < 16; e++) o[t][e] *= f;
-                if (NC > 8) asm volatile("" : "+a"(o[t]));
+                if (ACC) asm volatile("" : "+a"(o[t]));
             }
         }
         // weights: 2^8 e^(x - m) sv 2^-eref in fp16
@@ -956,7 +961,7 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 ? 8 / WV : 1) void k_kv8_tile(Kv8A
             k = 1.f;
             off = lr;
         }
-        f16x2 p[2][8];
+        f16x2 p[PARTS][2][8];
         float sum = 0.f;
         const f16x2 one = {(_Float16) 1.f, (_Float16) 1.f};
 #pragma unroll
@@ -967,8 +972,12 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 ? 8 / WV : 1) void k_kv8_tile(Kv8A
 #pragma unroll
                 for (int v = 0; v < 2; v++)
                     y[v] = __builtin_amdgcn_exp2f(MASK ? fmaf(sc[T][2 * e + v] - base, LOG2E, lr) : fmaf(sc[T][2 * e + v], k, off));
-                p[T][e] = __builtin_convertvector(y, f16x2);
-                sum = __builtin_amdgcn_fdot2(p[T][e], one, sum, false);
+                p[0][T][e] = __builtin_convertvector(y, f16x2);
+                sum = __builtin_amdgcn_fdot2(p[0][T][e], one, sum, false);
+                if (F32) {
+                    p[PARTS - 1][T][e] = __builtin_convertvector(y - __builtin_convertvector(p[0][T][e], f32x2), f16x2);
+                    sum = __builtin_amdgcn_fdot2(p[PARTS - 1][T][e], one, sum, false);
+                }
             }
         l = fmaf(sum, __builtin_amdgcn_exp2f(-lr), l);
         if (poison && mine.lo < t0 + KV8_PAGE && mine.hi > t0) l = nan;
@@ -976,13 +985,17 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 ? 8 / WV : 1) void k_kv8_tile(Kv8A
         for (int T = 0; T < 2; T++)
 #pragma unroll
             for (int v = 0; v < 2; v++) {
-                f16x8 b;
+                f16x8 b[PARTS];
 #pragma unroll
-                for (int e = 0; e < 8; e++) b[e] = p[T][2 * (v + 2 * (e >> 2)) + ((e & 3) >> 1)][e & 1];
+                for (int y = 0; y < PARTS; y++)
 #pragma unroll
-                for (int t = 0; t < ND; t++)
-                    o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                        __builtin_bit_cast(f16x8, cur[(2 * NC + t * 4 + T * 2 + v) * 64 + lane]), b, o[t], 0, 0, 0);
+                    for (int e = 0; e < 8; e++) b[y][e] = p[y][T][2 * (v + 2 * (e >> 2)) + ((e & 3) >> 1)][e & 1];
+#pragma unroll
+                for (int t = 0; t < ND; t++) {
+                    const f16x8 c = __builtin_bit_cast(f16x8, cur[(2 * NC + t * 4 + T * 2 + v) * 64 + lane]);
+#pragma unroll
+                    for (int y = 0; y < PARTS; y++) o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(c, b[y], o[t], 0, 0, 0);
+                }
             }
     }
     if (KS > 1) {                             // the groups meet in the first, through LDS, in units of 2^m and 2^eref
@@ -1044,7 +1057,8 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 ? 8 / WV : 1) void k_kv8_tile(Kv8A
             if (32 * t + 8 * e >= D) continue;
             const int d = 32 * t + 8 * e + 4 * half;
             const float4 y = make_float4(o[t][4 * e] * f, o[t][4 * e + 1] * f, o[t][4 * e + 2] * f, o[t][4 * e + 3] * f);
-            if (a.nch > 1) *(float4 *) (a.ws + (at * a.nch + c) * D + d) = y;
+            if (F32 && a.nch == 1) *(float4 *) ((float *) a.out + at * D + d) = y;
+            else if (a.nch > 1) *(float4 *) (a.ws + (at * a.nch + c) * D + d) = y;
             else *(uint2 *) ((uint16_t *) a.out + at * D + d) =
                 make_uint2(pack_bf16(y.x, y.y), pack_bf16(y.z, y.w));
         }
@@ -1156,12 +1170,12 @@ struct AttnPlan { bool tile; int RS, ngrp, C, nch, fold, wv, ks, sw; bool nt; };
 AttnPlan attn_plan(int f32, int Hq, int D, int Hkv, int nseq, int max_n, int max_len, int window) {
     AttnPlan p;
     const int64_t rows = (int64_t) max_n * (Hq / Hkv);
-    p.tile = !f32 && rows > 16;
+    p.tile = rows > 16 && (!f32 || D <= 128);                    // (fp32 at D > 128 has no registers for two parts of q)
     p.RS = rows <= 4 ? 1 : (rows <= 8 || D > 64 ? 2 : 4);        // (four sets' registers fit beside the codes of D = 64)
     // The prompt kernel's workgroups: 8 waves over 256 rows where every row sees nearly the same tokens, 8 waves in two
     // groups over 128 rows where there are no more, else 4 waves over 128 rows, which balance a causal triangle better.
     // (8 waves need whole units of a page: D up to 64 and from 97 to 128.)
-    const bool eight = D <= 64 || (D > 96 && D <= 128);
+    const bool eight = !f32 && (D <= 64 || (D > 96 && D <= 128));
     p.wv = eight && (rows <= 128 || (int64_t) max_n * 4 <= max_len) ? 8 : 4;
     p.ks = p.wv == 8 && rows <= 128 ? 2 : 1;
     const int group = p.tile ? 32 * p.wv / p.ks : 4 * p.RS;
@@ -1169,11 +1183,16 @@ AttnPlan attn_plan(int f32, int Hq, int D, int Hkv, int nseq, int max_n, int max
     const int64_t wgs = (int64_t) Hkv * p.ngrp * nseq, eff = window > 0 && window + max_n < max_len ? window + max_n : max_len;
     int64_t C;
     if (p.tile) {
-        // split along the tokens where the workgroups leave CUs without, in chunks of 512 or more; not for twofold gains,
-        // which the partials and the join cost again
-        const int64_t slots = p.wv == 8 || D > 128 ? 256 : 512;
-        int64_t nch = slots / wgs >= 3 ? slots / wgs : 1, most = (max_len + 511) / 512;
-        nch = nch > most ? most : nch;
+        // Split along the tokens where the workgroups leave CUs without, in chunks of 512 tokens or more (2048 for a twofold
+        // split, whose gain the partials and the join cost again: 1024 tokens on themselves 34 us whole, 31 + 22 in two),
+        // and further where whole rounds of the workgroups come out fuller.
+        const int64_t slots = p.wv == 8 || D > 128 || f32 ? 256 : 512;
+        auto used = [&](int64_t n) { return (double) (wgs * n) / (double) ((wgs * n + slots - 1) / slots * slots); };
+        int64_t nch = std::min<int64_t>(std::max<int64_t>(slots / wgs, 1), (max_len + 511) / 512);
+        if (nch == 2 && max_len < 4096) nch = 1;
+        if ((int64_t) max_n * 4 <= max_len)
+            for (int64_t n = nch + 1; n <= 8 && max_len / n >= 2048; n++)
+                if (used(n) > 1.15 * used(nch)) nch = n;
         C = ((max_len + nch - 1) / nch + KV8_PAGE - 1) / KV8_PAGE * KV8_PAGE;
     } else {
         const int64_t single = 2048;
@@ -1213,14 +1232,20 @@ template <int NC> hipError_t run_attn(const Kv8AttnArgs & a, const AttnPlan & p,
     const size_t lds = 2 * 4 * NC * 1024;
     if constexpr (NC <= 8 && NC % 4 == 0)
         if (p.wv == 8) {
-            if (p.ks == 2 && a.mask) k_kv8_tile<NC, 8, 2, true><<<grid, 512, 2 * lds, s>>>(a);
-            else if (p.ks == 2) k_kv8_tile<NC, 8, 2, false><<<grid, 512, 2 * lds, s>>>(a);
-            else if (a.mask) k_kv8_tile<NC, 8, 1, true><<<grid, 512, lds, s>>>(a);
-            else k_kv8_tile<NC, 8, 1, false><<<grid, 512, lds, s>>>(a);
+            if (p.ks == 2 && a.mask) k_kv8_tile<NC, 8, 2, true, false><<<grid, 512, 2 * lds, s>>>(a);
+            else if (p.ks == 2) k_kv8_tile<NC, 8, 2, false, false><<<grid, 512, 2 * lds, s>>>(a);
+            else if (a.mask) k_kv8_tile<NC, 8, 1, true, false><<<grid, 512, lds, s>>>(a);
+            else k_kv8_tile<NC, 8, 1, false, false><<<grid, 512, lds, s>>>(a);
             return hipGetLastError();
         }
-    if (a.mask) k_kv8_tile<NC, 4, 1, true><<<grid, KT, lds, s>>>(a);
-    else k_kv8_tile<NC, 4, 1, false><<<grid, KT, lds, s>>>(a);
+    if constexpr (NC <= 8)
+        if (a.f32) {
+            if (a.mask) k_kv8_tile<NC, 4, 1, true, true><<<grid, KT, lds, s>>>(a);
+            else k_kv8_tile<NC, 4, 1, false, true><<<grid, KT, lds, s>>>(a);
+            return hipGetLastError();
+        }
+    if (a.mask) k_kv8_tile<NC, 4, 1, true, false><<<grid, KT, lds, s>>>(a);
+    else k_kv8_tile<NC, 4, 1, false, false><<<grid, KT, lds, s>>>(a);
     return hipGetLastError();
 }
 
