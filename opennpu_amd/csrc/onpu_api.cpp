@@ -1907,7 +1907,7 @@ static bool kv8_fill(const char * name, const void * codes, const float * scales
                      const int32_t * table, int64_t tld, int P, const int32_t * pos, const int32_t * off, int nseq, int64_t T,
                      int max_n, Kv8Cache & c, Kv8Table & t) {
     const char * why = nullptr;
-    if (!codes || !scales || !table || !pos) why = "a null pointer";
+    if (!codes || !scales || !table || !pos) why = "pointers that are not null";
     else if (D <= 0 || D > KV8_MAX_D || D % 16 != 0) why = "D a multiple of 16 up to 256";
     else if (Hkv <= 0 || pages <= 0 || pages > INT32_MAX) why = "Hkv and pages positive, pages below 2^31";
     else if (((uintptr_t) codes % 16) || ((uintptr_t) scales % 8)) why = "codes 16-byte aligned, scales 8-byte aligned";
@@ -1937,10 +1937,10 @@ static int kv8_done(const char * name, hipError_t e) {
 int onpu_kv8_write_dev(void * codes, float * scales, int64_t pages, int Hkv, int D, const void * k, const void * v,
                        int kv_bf16, int64_t krs, int64_t khs, int64_t vrs, int64_t vhs, const int32_t * table, int64_t tld,
                        int P, const int32_t * pos, const int32_t * off, int nseq, int64_t T, int max_n, void * stream) {
+    if (T == 0 && nseq >= 0) return 0;                           // no rows (an empty table may have no address)
     Kv8Cache c;
     Kv8Table t;
     if (!kv8_fill("onpu_kv8_write_dev", codes, scales, pages, Hkv, D, table, tld, P, pos, off, nseq, T, max_n, c, t)) return -1;
-    if (T == 0) return 0;
     const int b = kv_bf16 ? 2 : 4;
     if (T == 1) krs = vrs = 0;                                   // (the stride of one row or head means nothing)
     if (Hkv == 1) khs = vhs = 0;
@@ -1955,10 +1955,10 @@ int onpu_kv8_write_dev(void * codes, float * scales, int64_t pages, int Hkv, int
 int onpu_kv8_read_dev(const void * codes, const float * scales, int64_t pages, int Hkv, int D, const int32_t * table,
                       int64_t tld, int P, const int32_t * pos, const int32_t * off, int nseq, int64_t T, int max_n, void * k,
                       void * v, int kv_bf16, void * stream) {
+    if (T == 0 && nseq >= 0) return 0;                           // no rows (an empty table may have no address)
     Kv8Cache c;
     Kv8Table t;
     if (!kv8_fill("onpu_kv8_read_dev", codes, scales, pages, Hkv, D, table, tld, P, pos, off, nseq, T, max_n, c, t)) return -1;
-    if (T == 0) return 0;
     if ((kv_bf16 != 0 && kv_bf16 != 1) || !kv8_rows_ok(k, 0, 0, 4) || !kv8_rows_ok(v, 0, 0, 4)) {
         set_err("onpu_kv8_read_dev: needs k and v fp32 or bf16, 16-byte aligned");
         return -1;
@@ -1977,10 +1977,10 @@ int onpu_kv8_attn_dev(const void * q, int q_bf16, int Hq, int64_t qrs, int64_t q
                       int64_t pages, int Hkv, int D, const int32_t * table, int64_t tld, int P, const int32_t * lens,
                       const int32_t * off, int nseq, int64_t T, int max_n, int max_len, const float * mask, int64_t mld,
                       const float * sinks, int window, float scale, void * out, void * ws, int64_t ws_bytes, void * stream) {
+    if (T == 0 && nseq >= 0) return 0;                           // no rows (an empty table may have no address)
     Kv8Cache c;
     Kv8Table t;
     if (!kv8_fill("onpu_kv8_attn_dev", codes, scales, pages, Hkv, D, table, tld, P, lens, off, nseq, T, max_n, c, t)) return -1;
-    if (T == 0) return 0;
     if (Hq <= 0 || Hq % Hkv || max_len < 1 || max_len > INT32_MAX - 64 || window < 0 || (mask && mld < max_len)) {
         set_err("onpu_kv8_attn_dev: needs Hq a multiple of Hkv, max_len from 1 to 2^31 - 65, window >= 0, mask rows of max_len or more");
         return -1;

@@ -28,15 +28,17 @@ ONPU_HD int kv8_v_at(int D, int token, int d) {
 }
 
 // The tokens of sequence i of a call: rows [row, row + n) of its T. off may hold anything: rows stay
-// inside [0, T) and n inside [0, max_n]. Without off every sequence has max_n rows.
-struct Kv8Rows { int64_t row; int n; };
+// inside [0, T) and n inside [0, max_n]; all: the sequence's rows, also where they are more than max_n.
+// Without off every sequence has max_n rows.
+struct Kv8Rows { int64_t row, all; int n; };
 ONPU_HD Kv8Rows kv8_rows(const int32_t * off, int i, int64_t T, int max_n) {
     Kv8Rows r;
-    if (!off) { r.row = (int64_t) i * max_n; r.n = max_n; return r; }
+    if (!off) { r.row = (int64_t) i * max_n; r.all = r.n = max_n; return r; }
     int64_t a = off[i], b = off[i + 1];
     a = a < 0 ? 0 : (a > T ? T : a);
     b = b < a ? a : (b > T ? T : b);
     r.row = a;
+    r.all = b - a;
     r.n = (int) (b - a > max_n ? max_n : b - a);
     return r;
 }

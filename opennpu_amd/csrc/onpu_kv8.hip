@@ -423,7 +423,7 @@ __global__ __launch_bounds__(64 * SW, SW == 8 ? 2 : (RS == 1 ? (NC <= 4 ? 4 : (N
     if (R0 >= rows) return;
     const int nrow = rows - R0 < HG ? rows - R0 : HG;
     const int full = a.t.pos[i] < 0 ? 0 : a.t.pos[i], len = full < a.max_len ? full : a.max_len;
-    const int64_t at0 = (int64_t) full - r.n;
+    const int64_t at0 = (int64_t) full - r.all;
     const Kv8Seen first = kv8_seen(at0 + R0 / a.rep, len, a.window), last = kv8_seen(at0 + (R0 + nrow - 1) / a.rep, len, a.window);
     const int64_t c0 = (int64_t) c * a.C, c1 = c0 + a.C;
     const int lo = first.lo > c0 ? first.lo : (int) (c0 < last.hi ? c0 : last.hi), hi = last.hi < c1 ? last.hi : (int) c1;
@@ -728,7 +728,7 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 && !F32 ? 8 / WV : 1) void k_kv8_t
     z = a.fold && z >= ngrp / 2 ? z - ngrp / 2 : ngrp - 1 - z;
     const int R0 = z * TR, nrow = rows - R0 < TR ? rows - R0 : TR;
     const int full = a.t.pos[i] < 0 ? 0 : a.t.pos[i], len = full < a.max_len ? full : a.max_len;
-    const int64_t at0 = (int64_t) full - r.n;
+    const int64_t at0 = (int64_t) full - r.all;
     const Kv8Seen first = kv8_seen(at0 + R0 / a.rep, len, a.window), last = kv8_seen(at0 + (R0 + nrow - 1) / a.rep, len, a.window);
     const int64_t c0 = (int64_t) c * a.C, c1 = c0 + a.C;
     const int lo = first.lo > c0 ? first.lo : (int) (c0 < last.hi ? c0 : last.hi), hi = last.hi < c1 ? last.hi : (int) c1;
@@ -848,8 +848,7 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 && !F32 ? 8 / WV : 1) void k_kv8_t
     for (int n = 0; n < rounds; n++) {
         const int t0 = (p0 + n * KS) * KV8_PAGE, n2 = n + 2;
         const uint4 * cur = page + (n & 1) * FRAGS * 64;
-        const float skc = sk;
-        float lsc = ls;
+        float skc = sk, lsc = ls;
         if ((n2 & 63) == 0 && n2 < np) fetch(p0 + n2 * KS);
         lds_barrier();                                           // cur is whole, the other buffer is read
         const bool skip = !live || n >= np || t0 >= wlast.hi || t0 + KV8_PAGE <= wfirst.lo;
@@ -891,6 +890,9 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 && !F32 ? 8 / WV : 1) void k_kv8_t
             }
         }
         if (skip) continue;
+        // a page of a NaN scale: rows that see it become NaN at its end; with the scale in their scores the others would, too
+        const bool poison = !(lsc < 128.f) || skc != skc;
+        if (skc != skc) skc = 1.f;
         const float cs0 = rowf * skc, cs = cs0 < 1e-35f ? 1e-35f : cs0;      // (above 0, so that -inf stays -inf; a NaN stays)
         const bool edge = t0 < wlast.lo || t0 + KV8_PAGE > wfirst.hi || t0 < lo || t0 + KV8_PAGE > hi;
         if (MASK) {
@@ -921,8 +923,7 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 && !F32 ? 8 / WV : 1) void k_kv8_t
         }
         if (!MASK) mx *= cs;
         // V's scale as a power of two within 2^4 of the reference, which moves otherwise (never 2^60 below the largest)
-        const bool poison = !(lsc < 128.f);
-        if (poison) lsc = eref > -1000 ? (float) eref : 0.f;
+        if (!(lsc < 128.f)) lsc = eref > -1000 ? (float) eref : 0.f;
         const float step = MASK ? 3.f / LOG2E : 3.f;
         const bool move = mx > m + step || (m == -inf && mx > m);
         const bool shift = fabsf(lsc - (float) eref) > 4.f;
@@ -1079,7 +1080,7 @@ __global__ __launch_bounds__(KT) void k_kv8_combine(Kv8AttnArgs a) {
     const bool live = j < r.n;
     if (W == 1 ? !live : (blockIdx.x * (CW / W)) / a.Hq >= r.n) return;       // (W > 1 meets at a barrier: leave together)
     const int full = a.t.pos[i] < 0 ? 0 : a.t.pos[i], len = full < a.max_len ? full : a.max_len;
-    const Kv8Seen s = kv8_seen((int64_t) full - r.n + j, len, a.window);
+    const Kv8Seen s = kv8_seen((int64_t) full - r.all + j, len, a.window);
     const int ca = s.lo / a.C, cb = live && s.hi > s.lo ? (s.hi - 1) / a.C + 1 : ca;         // the chunks that this row sees
     const int64_t o = (r.row + (live ? j : 0)) * a.Hq + h;
     const float * wo = a.ws + o * a.nch * D, * wml = a.ws + a.t.T * a.Hq * a.nch * D + o * a.nch * 2;
@@ -1131,7 +1132,7 @@ __global__ __launch_bounds__(KT) void k_kv8_join(Kv8AttnArgs a) {
     const Kv8Rows r = kv8_rows(a.t.off, i, a.t.T, a.t.max_n);
     if (j >= r.n) return;
     const int full = a.t.pos[i] < 0 ? 0 : a.t.pos[i], len = full < a.max_len ? full : a.max_len;
-    const Kv8Seen s = kv8_seen((int64_t) full - r.n + j, len, a.window);
+    const Kv8Seen s = kv8_seen((int64_t) full - r.all + j, len, a.window);
     const int ca = s.lo / a.C, n = s.hi > s.lo ? (s.hi - 1) / a.C + 1 - ca : 0;         // the chunks that this row sees
     const int64_t o = (r.row + j) * a.Hq + h;
     const float * wo = a.ws + (o * a.nch + ca) * D + d, * wml = a.ws + a.t.T * a.Hq * a.nch * D + (o * a.nch + ca) * 2;

@@ -268,28 +268,22 @@ def _kv8_refuse(codes, scales, table, pos, off, vals, what, here):
     raise ValueError(f"{what}: rows must be fp32 or bf16 [T][heads][{codes.shape[3] // 64}] with unit stride in the last dimension")
 
 
-def _kv8(codes, scales, table, pos, off, vals, what):
+def _kv8(codes, scales, table, pos, off, rows, what):
     """the cache's, table's and row ranges' arguments, checked (in one expression: a decode step's call is bound
-    by its issue); vals: (fp32 or bf16 [T][heads][D] tensor, ...). Returns pages, Hkv, D, sequences, P, the GPU"""
+    by its issue); rows: fp32 or bf16 [T][heads][D]. Returns pages, Hkv, D, sequences, P, the GPU, whether bf16"""
     import torch
-    f32, i32, bf16 = torch.float32, torch.int32, torch.bfloat16
-    here = torch.cuda.current_device()
-    cs, ts = codes.shape, table.shape
-    ok = (codes.dtype is torch.int8 and len(cs) == 4 and cs[2] == 2 and cs[3] % 64 == 0 and scales.dtype is f32
-          and scales.shape == cs[:3] and table.dtype is i32 and len(ts) == 2 and (ts[1] <= 1 or table.stride(1) == 1)
-          and pos.dtype is i32 and pos.shape == ts[:1] and codes.is_contiguous() and scales.is_contiguous()
-          and pos.is_contiguous() and codes.get_device() == here == scales.get_device() == table.get_device() == pos.get_device())
-    if off is not None:
-        ok = ok and off.dtype is i32 and off.shape == (ts[0] + 1,) and off.is_contiguous() and off.get_device() == here
-    D = cs[-1] // 64
-    for t in vals:
-        if not ok:
-            break
-        shape = t.shape
-        ok = len(shape) == 3 and shape[2] == D and t.stride(2) == 1 and t.get_device() == here and (t.dtype is f32 or t.dtype is bf16)
-    if not ok:
-        _kv8_refuse(codes, scales, table, pos, off, vals, what, here)
-    return cs[0], cs[1], D, ts[0], ts[1], here
+    here = torch._C._cuda_getDevice()
+    cs, ts, dt = codes.shape, table.shape, rows.dtype
+    bf16 = dt is torch.bfloat16
+    if (len(cs) == 4 and len(ts) == 2 and rows.dim() == 3 and cs[2] == 2 and 64 * rows.size(2) == cs[3] and rows.stride(2) == 1
+            and (bf16 or dt is torch.float32) and codes.dtype is torch.int8 and scales.dtype is torch.float32
+            and table.dtype is torch.int32 and pos.dtype is torch.int32 and scales.shape == cs[:3] and pos.shape == ts[:1]
+            and (ts[1] <= 1 or table.stride(1) == 1) and codes.is_contiguous() and scales.is_contiguous() and pos.is_contiguous()
+            and here == codes.get_device() == scales.get_device() == table.get_device() == pos.get_device() == rows.get_device()
+            and (off is None or (off.dtype is torch.int32 and off.dim() == 1 and off.size(0) == ts[0] + 1 and off.is_contiguous()
+                                 and off.get_device() == here))):
+        return cs[0], cs[1], cs[3] // 64, ts[0], ts[1], here, bf16
+    _kv8_refuse(codes, scales, table, pos, off, (rows,), what, here)
 
 
 def _kv8_n(T, nseq, off, max_n, what):
@@ -301,27 +295,22 @@ def _kv8_n(T, nseq, off, max_n, what):
     return T if max_n is None else int(max_n)
 
 
-def _raw_stream(here):
-    import torch
-    return torch._C._cuda_getCurrentRawStream(here)
-
-
 def kv8_write(codes, scales, k, v, table, pos, off=None, max_n=None):
     """Quantise k, v (fp32 or bf16 [T][Hkv][D]) into the cache's pages (onpu_kv8_write_dev): sequence i's
     rows off[i]:off[i + 1] (off None: T / sequences each) go to positions pos[i], pos[i] + 1, ...; max_n: the most
     rows of one sequence (default: as many as there are)."""
     import torch
     L = require_gpu()
-    pages, Hkv, D, nseq, P, here = _kv8(codes, scales, table, pos, off, (k, v), "kv8_write")
+    pages, Hkv, D, nseq, P, here, bf16 = _kv8(codes, scales, table, pos, off, k, "kv8_write")
     T, heads, _ = k.shape
-    if k.shape != v.shape or k.dtype is not v.dtype or heads != Hkv:
-        raise ValueError("kv8_write: k and v must have the same type and shape [T][Hkv][D]")
     krs, khs, _ = k.stride()
-    vrs, vhs, _ = v.stride()
-    check(L.onpu_kv8_write_dev(codes.data_ptr(), scales.data_ptr(), pages, Hkv, D, k.data_ptr(), v.data_ptr(),
-                               k.dtype is torch.bfloat16, krs, khs, vrs, vhs, table.data_ptr(), table.stride(0), P,
-                               pos.data_ptr(), None if off is None else off.data_ptr(), nseq, T,
-                               _kv8_n(T, nseq, off, max_n, "kv8_write"), _raw_stream(here)), "kv8_write")
+    vrs, vhs, unit = v.stride() if v.dim() == 3 else (0, 0, 0)
+    if k.shape != v.shape or k.dtype is not v.dtype or heads != Hkv or unit != 1 or v.get_device() != here:
+        raise ValueError("kv8_write: k and v must have the same type and shape [T][Hkv][D], unit strides, and be on one GPU")
+    check(L.onpu_kv8_write_dev(codes.data_ptr(), scales.data_ptr(), pages, Hkv, D, k.data_ptr(), v.data_ptr(), bf16, krs, khs,
+                               vrs, vhs, table.data_ptr(), table.stride(0), P, pos.data_ptr(),
+                               None if off is None else off.data_ptr(), nseq, T, _kv8_n(T, nseq, off, max_n, "kv8_write"),
+                               torch._C._cuda_getCurrentRawStream(here)), "kv8_write")
 
 
 def kv8_read(codes, scales, table, pos, rows, off=None, max_n=None, dtype=None, out=None):
@@ -329,22 +318,24 @@ def kv8_read(codes, scales, table, pos, rows, off=None, max_n=None, dtype=None, 
     [rows][Hkv][D], bf16 (the default) or fp32; rows in all, off and max_n as kv8_write."""
     import torch
     L = require_gpu()
-    pages, Hkv, D, nseq, P, here = _kv8(codes, scales, table, pos, off, () if out is None else tuple(out), "kv8_read")
     if out is None:
         dtype = dtype or torch.bfloat16
         if dtype is not torch.float32 and dtype is not torch.bfloat16:
             raise ValueError("kv8_read: dtype must be fp32 or bf16")
-        k = codes.new_empty((rows, Hkv, D), dtype=dtype)
-        v = torch.empty_like(k)
+        # k, then v of one allocation (a row's values are a multiple of 16, so both start on 32 bytes)
+        k, v = codes.new_empty((2, rows, codes.size(1), codes.size(-1) // 64), dtype=dtype).unbind(0)
     else:
         k, v = out
-        if k.shape != (rows, Hkv, D) or v.shape != k.shape or k.dtype != v.dtype or not (k.is_contiguous() and v.is_contiguous()) \
+        if v.shape != k.shape or k.dtype != v.dtype or not (k.is_contiguous() and v.is_contiguous()) or k.device != v.device \
                 or dtype not in (None, k.dtype):
             raise ValueError("kv8_read: out must be two contiguous [rows][Hkv][D] tensors of one type")
+    pages, Hkv, D, nseq, P, here, bf16 = _kv8(codes, scales, table, pos, off, k, "kv8_read")
+    if out is not None and k.shape != (rows, Hkv, D):
+        raise ValueError("kv8_read: out must be two contiguous [rows][Hkv][D] tensors of one type")
     check(L.onpu_kv8_read_dev(codes.data_ptr(), scales.data_ptr(), pages, Hkv, D, table.data_ptr(), table.stride(0), P,
                               pos.data_ptr(), None if off is None else off.data_ptr(), nseq, rows,
-                              _kv8_n(rows, nseq, off, max_n, "kv8_read"), k.data_ptr(), v.data_ptr(),
-                              k.dtype is torch.bfloat16, _raw_stream(here)), "kv8_read")
+                              _kv8_n(rows, nseq, off, max_n, "kv8_read"), k.data_ptr(), v.data_ptr(), bf16,
+                              torch._C._cuda_getCurrentRawStream(here)), "kv8_read")
     return k, v
 
 
@@ -358,20 +349,25 @@ def kv8_attn(q, codes, scales, table, lens, off=None, max_n=None, max_len=None, 
     per call in flight (default: torch's allocator). Returns out [T][Hq][D] in q's type."""
     import torch
     L = require_gpu()
-    pages, Hkv, D, nseq, P, here = _kv8(codes, scales, table, lens, off, (q,) if out is None else (q, out), "kv8_attn")
+    pages, Hkv, D, nseq, P, here, bf16 = _kv8(codes, scales, table, lens, off, q, "kv8_attn")
     T, Hq, _ = q.shape
     qrs, qhs, _ = q.stride()
-    bf16 = q.dtype is torch.bfloat16
     n = _kv8_n(T, nseq, off, max_n, "kv8_attn")
     max_len = 64 * P if max_len is None else int(max_len)
     if out is None:
         out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
-        raise ValueError("kv8_attn: out must be contiguous, of q's shape and type")
-    for t, shape in ((mask, None), (sinks, (Hq,))):
-        if t is not None and (t.dtype != torch.float32 or t.get_device() != here or t.stride(-1) != 1
-                              or (t.shape != shape if shape else t.dim() != 2 or t.shape[0] != nseq or t.shape[1] < max_len)):
-            raise ValueError("kv8_attn: mask must be fp32 [sequences][>= max_len], sinks fp32 [Hq], on q's GPU")
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.get_device() != here:
+        raise ValueError("kv8_attn: out must be contiguous, of q's shape and type, on q's GPU")
+    mp = ml = sp = None
+    if mask is not None:
+        if mask.dtype != torch.float32 or mask.dim() != 2 or mask.shape[0] != nseq or mask.shape[1] < max_len \
+                or mask.stride(1) != 1 or mask.get_device() != here:
+            raise ValueError("kv8_attn: mask must be fp32 [sequences][>= max_len] on q's GPU, rows of unit stride")
+        mp, ml = mask.data_ptr(), mask.stride(0) if nseq > 1 else mask.shape[1]
+    if sinks is not None:
+        if sinks.dtype != torch.float32 or sinks.shape != (Hq,) or not sinks.is_contiguous() or sinks.get_device() != here:
+            raise ValueError("kv8_attn: sinks must be fp32 [Hq] on q's GPU, contiguous")
+        sp = sinks.data_ptr()
     if ws is None:
         nb = L.onpu_kv8_attn_ws_bytes(bf16, Hq, D, Hkv, nseq, T, n, max_len, window)
         if nb:
@@ -380,8 +376,7 @@ def kv8_attn(q, codes, scales, table, lens, off=None, max_n=None, max_len=None, 
         raise ValueError("kv8_attn: ws must be contiguous, on q's GPU")
     check(L.onpu_kv8_attn_dev(q.data_ptr(), bf16, Hq, qrs, qhs, codes.data_ptr(), scales.data_ptr(), pages, Hkv, D,
                               table.data_ptr(), table.stride(0), P, lens.data_ptr(), None if off is None else off.data_ptr(),
-                              nseq, T, n, max_len, None if mask is None else mask.data_ptr(),
-                              0 if mask is None else mask.stride(0), None if sinks is None else sinks.data_ptr(), window,
-                              D ** -0.5 if scale is None else scale, out.data_ptr(), None if ws is None else ws.data_ptr(),
-                              0 if ws is None else ws.nbytes, _raw_stream(here)), "kv8_attn")
+                              nseq, T, n, max_len, mp, ml or 0, sp, window, D ** -0.5 if scale is None else scale,
+                              out.data_ptr(), None if ws is None else ws.data_ptr(), 0 if ws is None else ws.nbytes,
+                              torch._C._cuda_getCurrentRawStream(here)), "kv8_attn")
     return out

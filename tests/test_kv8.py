@@ -15,7 +15,7 @@ SRC = """
 #include "onpu_kv8.h"
 extern "C" {
 int at(int kv, int D, int token, int d) { return kv ? kv8_v_at(D, token, d) : kv8_k_at(D, token, d); }
-void rows(const int32_t * off, int i, int64_t T, int max_n, int64_t * o) { Kv8Rows r = kv8_rows(off, i, T, max_n); o[0] = r.row; o[1] = r.n; }
+void rows(const int32_t * off, int i, int64_t T, int max_n, int64_t * o) { Kv8Rows r = kv8_rows(off, i, T, max_n); o[0] = r.row; o[1] = r.n; o[2] = r.all; }
 int page(const int32_t * table, int64_t p, int P, int pages) { return kv8_page(table, p, P, pages); }
 void seen(int64_t at, int len, int window, int * o) { Kv8Seen s = kv8_seen(at, len, window); o[0] = s.lo; o[1] = s.hi; }
 }
@@ -45,7 +45,7 @@ def test_layout(host, D):
 
 def test_row_ranges_stay_inside(host):
     """whatever off holds, rows [row, row + n) lie in [0, T) and n in [0, max_n]"""
-    out = (C.c_int64 * 2)()
+    out = (C.c_int64 * 3)()
     big = 2 ** 31 - 1
     for T in (1, 7, 100):
         for a in (-big - 1, -1, 0, 3, 7, 100, big):
@@ -53,12 +53,12 @@ def test_row_ranges_stay_inside(host):
                 off = np.array([a, b], np.int32)
                 for max_n in (1, 5, big):
                     host.rows(off.ctypes.data, 0, T, max_n, out)
-                    row, n = out
-                    assert 0 <= row <= T and 0 <= n <= max_n and row + n <= T
+                    row, n, every = out
+                    assert 0 <= row <= T and 0 <= n <= max_n and row + every <= T and n == min(every, max_n)
                     if 0 <= a <= b <= T:
                         assert row == a and n == min(b - a, max_n)
     host.rows(None, 3, 20, 5, out)
-    assert tuple(out) == (15, 5)
+    assert tuple(out) == (15, 5, 5)
 
 
 def test_pages_that_do_not_exist(host):

@@ -492,8 +492,47 @@ def test_attn_strided_queries_and_untouched_rows(gpu):
     want = kv8_attn(q.contiguous(), *args, max_n=3)
     assert torch.equal(out[:5], want[:5]) and (out[5:] == 7).all()
     out.fill_(7)
-    kv8_attn(q, *args, max_n=2, out=out)
-    assert torch.equal(out[:2], want[:2]) and (out[4:] == 7).all()
+    kv8_attn(q, *args, max_n=2, out=out)                         # (the positions stay those of all three rows)
+    assert torch.equal(out[:4], want[:4]) and (out[4:] == 7).all()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_attn_many_pages_in_one_workgroup(gpu, dt):
+    """a sequence of more than 64 pages that is not split, beside short ones; one of its late pages holds a NaN
+    that the rows before it do not see, also where they share a wave with rows that do"""
+    rng = np.random.default_rng(21)
+    lens, n = [4500] + [30] * 39, [20] * 40
+
+    def spoil(table, codes, scales):
+        scales[table[0, 70], 3, 0] = np.nan                      # tokens 4480 ..: rows 0 .. of the last 20 do not see it
+        scales[table[0, 70], 5, 1] = np.nan
+    got, want, tol = _attn_case(rng, dt, 8, 8, 64, lens, n)
+    _close(got, want, tol)
+    for length, first in ((4490, 10), (4485, 15)):               # rows from `first` on see page 70
+        got, want, tol = _attn_case(rng, dt, 8, 8, 64, [length] + lens[1:], n, cache=spoil)
+        bad = np.isnan(got).any(-1)
+        assert bad[first:20, [3, 5]].all() and bad.sum() == 2 * (20 - first)
+        ok = ~np.isnan(got)
+        assert (np.abs(got - want)[ok] <= tol[ok]).all()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("n", [1, 40])
+def test_empty_calls(gpu, dt, n):
+    """no sequences, and no rows, are no error"""
+    import torch
+    from opennpu_amd.device import kv8_attn, kv8_cache, kv8_read, kv8_write
+    c, s = kv8_cache(2, 2, 64)
+    t, p = torch.empty((0, 3), dtype=torch.int32, device="cuda"), _i32([])
+    k = torch.empty((0, 2, 64), dtype=_dt(dt), device="cuda")
+    kv8_write(c, s, k, k, t, p)
+    assert kv8_read(c, s, t, p, 0)[0].shape == (0, 2, 64)
+    assert kv8_attn(torch.empty((0, 4, 64), dtype=_dt(dt), device="cuda"), c, s, t, p).shape == (0, 4, 64)
+    t, p, off = _i32([[0, 1]] * 2), _i32([0, 5]), _i32([0, 0, 0])
+    kv8_write(c, s, k, k, t, p, off, n)
+    out = torch.full((3, 4, 64), 7.0, dtype=_dt(dt), device="cuda")
+    kv8_attn(torch.zeros_like(out), c, s, t, p, off, n, out=out)
+    assert (out == 7).all() and (c == 0).all()
 
 
 def test_a_run_of_the_three(gpu):
