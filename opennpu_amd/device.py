@@ -12,7 +12,7 @@ import ctypes as C
 
 import numpy as np
 
-from ._lib import check, require_gpu
+from ._lib import LibraryMissing, check, require_gpu
 
 
 def _stream():
@@ -249,94 +249,37 @@ def kv8_cache(pages, Hkv, D, device=None):
             torch.zeros((pages, Hkv, 2), dtype=torch.float32, device=device or "cuda"))
 
 
-def _kv8_refuse(codes, scales, table, pos, off, vals, what, here):
-    """the reason why _kv8 does not take its arguments"""
-    import torch
-    if codes.dtype != torch.int8 or codes.dim() != 4 or codes.shape[2] != 2 or codes.shape[3] % 64 or not codes.is_contiguous():
-        raise ValueError(f"{what}: codes must be int8 [pages][Hkv][2][64 D], contiguous")
-    if scales.dtype != torch.float32 or scales.shape != codes.shape[:3] or not scales.is_contiguous():
-        raise ValueError(f"{what}: scales must be fp32 [pages][Hkv][2], contiguous")
-    if table.dtype != torch.int32 or table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
-        raise ValueError(f"{what}: table must be int32 [sequences][P] with rows of unit stride")
-    if pos.dtype != torch.int32 or pos.shape != table.shape[:1] or not pos.is_contiguous():
-        raise ValueError(f"{what}: positions or lengths must be int32, one per sequence, contiguous")
-    if off is not None and (off.dtype != torch.int32 or off.shape != (table.shape[0] + 1,) or not off.is_contiguous()):
-        raise ValueError(f"{what}: off must be int32, one more than the sequences, contiguous")
-    for t in (codes, scales, table, pos, off) + vals:
-        if t is not None and not (t.is_cuda and t.get_device() == here):
-            raise ValueError(f"{what}: every tensor must be on the current GPU (cuda:{here}), got {t.device}")
-    raise ValueError(f"{what}: rows must be fp32 or bf16 [T][heads][{codes.shape[3] // 64}] with unit stride in the last dimension")
+_KV8 = None
 
 
-def _kv8(codes, scales, table, pos, off, rows, what):
-    """the cache's, table's and row ranges' arguments, checked (in one expression: a decode step's call is bound
-    by its issue); rows: fp32 or bf16 [T][heads][D]. Returns pages, Hkv, D, sequences, P, the GPU, whether bf16"""
-    import torch
-    here = torch._C._cuda_getDevice()
-    cs, ts, dt = codes.shape, table.shape, rows.dtype
-    bf16 = dt is torch.bfloat16
-    if (len(cs) == 4 and len(ts) == 2 and rows.dim() == 3 and cs[2] == 2 and 64 * rows.size(2) == cs[3] and rows.stride(2) == 1
-            and (bf16 or dt is torch.float32) and codes.dtype is torch.int8 and scales.dtype is torch.float32
-            and table.dtype is torch.int32 and pos.dtype is torch.int32 and scales.shape == cs[:3] and pos.shape == ts[:1]
-            and (ts[1] <= 1 or table.stride(1) == 1) and codes.is_contiguous() and scales.is_contiguous() and pos.is_contiguous()
-            and here == codes.get_device() == scales.get_device() == table.get_device() == pos.get_device() == rows.get_device()
-            and (off is None or (off.dtype is torch.int32 and off.dim() == 1 and off.size(0) == ts[0] + 1 and off.is_contiguous()
-                                 and off.get_device() == here))):
-        return cs[0], cs[1], cs[3] // 64, ts[0], ts[1], here, bf16
-    _kv8_refuse(codes, scales, table, pos, off, (rows,), what, here)
-
-
-def _kv8_n(T, nseq, off, max_n, what):
-    """max_n: given, or the rows of each sequence (off None), or the most that one can have"""
-    if off is None:
-        if T % max(nseq, 1):
-            raise ValueError(f"{what}: {T} rows cannot be the same number for each of {nseq} sequences: give off")
-        return T // max(nseq, 1)
-    return T if max_n is None else int(max_n)
+def _kv8():
+    """opennpu_amd._kv8 (csrc/onpu_torch.cpp: the checks of the arguments and the calls, in C++ because a decode
+    step's calls are bound by their issue), with the loaded library's entries"""
+    global _KV8
+    if _KV8 is None:
+        L = require_gpu()
+        try:
+            from . import _kv8 as m
+        except ImportError as e:
+            raise LibraryMissing(f"opennpu_amd/_kv8.so is not built: run `python -m opennpu_amd.build` ({e})") from e
+        m.bind(*[C.cast(f, C.c_void_p).value for f in (L.onpu_kv8_write_dev, L.onpu_kv8_read_dev, L.onpu_kv8_attn_ws_bytes,
+                                                       L.onpu_kv8_attn_dev, L.onpu_last_error)])
+        _KV8 = m
+    return _KV8
 
 
 def kv8_write(codes, scales, k, v, table, pos, off=None, max_n=None):
     """Quantise k, v (fp32 or bf16 [T][Hkv][D]) into the cache's pages (onpu_kv8_write_dev): sequence i's
     rows off[i]:off[i + 1] (off None: T / sequences each) go to positions pos[i], pos[i] + 1, ...; max_n: the most
     rows of one sequence (default: as many as there are)."""
-    import torch
-    L = require_gpu()
-    pages, Hkv, D, nseq, P, here, bf16 = _kv8(codes, scales, table, pos, off, k, "kv8_write")
-    T, heads, _ = k.shape
-    krs, khs, _ = k.stride()
-    vrs, vhs, unit = v.stride() if v.dim() == 3 else (0, 0, 0)
-    if k.shape != v.shape or k.dtype is not v.dtype or heads != Hkv or unit != 1 or v.get_device() != here:
-        raise ValueError("kv8_write: k and v must have the same type and shape [T][Hkv][D], unit strides, and be on one GPU")
-    check(L.onpu_kv8_write_dev(codes.data_ptr(), scales.data_ptr(), pages, Hkv, D, k.data_ptr(), v.data_ptr(), bf16, krs, khs,
-                               vrs, vhs, table.data_ptr(), table.stride(0), P, pos.data_ptr(),
-                               None if off is None else off.data_ptr(), nseq, T, _kv8_n(T, nseq, off, max_n, "kv8_write"),
-                               torch._C._cuda_getCurrentRawStream(here)), "kv8_write")
+    (_KV8 or _kv8()).write(codes, scales, k, v, table, pos, off, max_n)
 
 
 def kv8_read(codes, scales, table, pos, rows, off=None, max_n=None, dtype=None, out=None):
     """The values of positions pos[i], pos[i] + 1, ... of every sequence (onpu_kv8_read_dev): k, v
     [rows][Hkv][D], bf16 (the default) or fp32; rows in all, off and max_n as kv8_write."""
-    import torch
-    L = require_gpu()
-    if out is None:
-        dtype = dtype or torch.bfloat16
-        if dtype is not torch.float32 and dtype is not torch.bfloat16:
-            raise ValueError("kv8_read: dtype must be fp32 or bf16")
-        # k, then v of one allocation (a row's values are a multiple of 16, so both start on 32 bytes)
-        k, v = codes.new_empty((2, rows, codes.size(1), codes.size(-1) // 64), dtype=dtype).unbind(0)
-    else:
-        k, v = out
-        if v.shape != k.shape or k.dtype != v.dtype or not (k.is_contiguous() and v.is_contiguous()) or k.device != v.device \
-                or dtype not in (None, k.dtype):
-            raise ValueError("kv8_read: out must be two contiguous [rows][Hkv][D] tensors of one type")
-    pages, Hkv, D, nseq, P, here, bf16 = _kv8(codes, scales, table, pos, off, k, "kv8_read")
-    if out is not None and k.shape != (rows, Hkv, D):
-        raise ValueError("kv8_read: out must be two contiguous [rows][Hkv][D] tensors of one type")
-    check(L.onpu_kv8_read_dev(codes.data_ptr(), scales.data_ptr(), pages, Hkv, D, table.data_ptr(), table.stride(0), P,
-                              pos.data_ptr(), None if off is None else off.data_ptr(), nseq, rows,
-                              _kv8_n(rows, nseq, off, max_n, "kv8_read"), k.data_ptr(), v.data_ptr(), bf16,
-                              torch._C._cuda_getCurrentRawStream(here)), "kv8_read")
-    return k, v
+    k, v = (None, None) if out is None else out
+    return (_KV8 or _kv8()).read(codes, scales, table, pos, rows, off, max_n, dtype, k, v)
 
 
 def kv8_attn(q, codes, scales, table, lens, off=None, max_n=None, max_len=None, mask=None, sinks=None, window=0, scale=None,
@@ -347,36 +290,4 @@ def kv8_attn(q, codes, scales, table, lens, off=None, max_n=None, max_len=None, 
     faster). mask fp32 [sequences][>= max_len] is added to the scores, sinks fp32 [Hq] is a logit per head without a
     value, window the last positions a query sees (0: all). ws: a workspace of onpu_kv8_attn_ws_bytes bytes, one
     per call in flight (default: torch's allocator). Returns out [T][Hq][D] in q's type."""
-    import torch
-    L = require_gpu()
-    pages, Hkv, D, nseq, P, here, bf16 = _kv8(codes, scales, table, lens, off, q, "kv8_attn")
-    T, Hq, _ = q.shape
-    qrs, qhs, _ = q.stride()
-    n = _kv8_n(T, nseq, off, max_n, "kv8_attn")
-    max_len = 64 * P if max_len is None else int(max_len)
-    if out is None:
-        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.get_device() != here:
-        raise ValueError("kv8_attn: out must be contiguous, of q's shape and type, on q's GPU")
-    mp = ml = sp = None
-    if mask is not None:
-        if mask.dtype != torch.float32 or mask.dim() != 2 or mask.shape[0] != nseq or mask.shape[1] < max_len \
-                or mask.stride(1) != 1 or mask.get_device() != here:
-            raise ValueError("kv8_attn: mask must be fp32 [sequences][>= max_len] on q's GPU, rows of unit stride")
-        mp, ml = mask.data_ptr(), mask.stride(0) if nseq > 1 else mask.shape[1]
-    if sinks is not None:
-        if sinks.dtype != torch.float32 or sinks.shape != (Hq,) or not sinks.is_contiguous() or sinks.get_device() != here:
-            raise ValueError("kv8_attn: sinks must be fp32 [Hq] on q's GPU, contiguous")
-        sp = sinks.data_ptr()
-    if ws is None:
-        nb = L.onpu_kv8_attn_ws_bytes(bf16, Hq, D, Hkv, nseq, T, n, max_len, window)
-        if nb:
-            ws = codes.new_empty((nb,))
-    elif ws.get_device() != here or not ws.is_contiguous():
-        raise ValueError("kv8_attn: ws must be contiguous, on q's GPU")
-    check(L.onpu_kv8_attn_dev(q.data_ptr(), bf16, Hq, qrs, qhs, codes.data_ptr(), scales.data_ptr(), pages, Hkv, D,
-                              table.data_ptr(), table.stride(0), P, lens.data_ptr(), None if off is None else off.data_ptr(),
-                              nseq, T, n, max_len, mp, ml or 0, sp, window, D ** -0.5 if scale is None else scale,
-                              out.data_ptr(), None if ws is None else ws.data_ptr(), 0 if ws is None else ws.nbytes,
-                              torch._C._cuda_getCurrentRawStream(here)), "kv8_attn")
-    return out
+    return (_KV8 or _kv8()).attn(q, codes, scales, table, lens, off, max_n, max_len, mask, sinks, window, scale, out, ws)
