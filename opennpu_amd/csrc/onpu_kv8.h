@@ -59,6 +59,12 @@ ONPU_HD Kv8Seen kv8_seen(int64_t at, int len, int window) {
     s.lo = lo < 0 ? 0 : (lo > s.hi ? s.hi : (int) lo);
     return s;
 }
+// the page-aligned position from which a sequence's chunks count: its first query at `at` sees nothing before it
+// (with a window the chunks are as many as the window needs, wherever it lies)
+ONPU_HD int kv8_start(int64_t at, int len, int window) {
+    const int lo = kv8_seen(at, len, window).lo;
+    return lo - lo % KV8_PAGE;
+}
 
 struct Kv8Cache {
     int8_t * codes;

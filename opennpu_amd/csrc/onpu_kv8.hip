@@ -425,7 +425,7 @@ __global__ __launch_bounds__(64 * SW, SW == 8 ? 2 : (RS == 1 ? (NC <= 4 ? 4 : (N
     const int full = a.t.pos[i] < 0 ? 0 : a.t.pos[i], len = full < a.max_len ? full : a.max_len;
     const int64_t at0 = (int64_t) full - r.all;
     const Kv8Seen first = kv8_seen(at0 + R0 / a.rep, len, a.window), last = kv8_seen(at0 + (R0 + nrow - 1) / a.rep, len, a.window);
-    const int64_t c0 = (int64_t) c * a.C, c1 = c0 + a.C;
+    const int64_t c0 = kv8_start(at0, len, a.window) + (int64_t) c * a.C, c1 = c0 + a.C;
     const int lo = first.lo > c0 ? first.lo : (int) (c0 < last.hi ? c0 : last.hi), hi = last.hi < c1 ? last.hi : (int) c1;
     if (a.nch > 1 && lo >= hi) return;
     const int pend = (hi + KV8_PAGE - 1) / KV8_PAGE;
@@ -715,7 +715,8 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 && !F32 ? 8 / WV : 1) void k_kv8_t
     static_assert(NU * WR == 2 * NC, "the waves share a page's units evenly");
     extern __shared__ __align__(16) uint4 lds4[];                // [KS][2][FRAGS][64]
     const int D = a.c.D, nc = D / 16, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int w = wave % WR, grp = wave / WR;                    // of KS groups of waves, each with every KS-th page
+    // of KS groups of waves, each with every KS-th page; waves 4 apart share a SIMD: the first 64 rows' are on all four
+    const int grp = wave / WR, w = (wave % WR) ^ (2 * grp);
     uint4 * page = lds4 + grp * 2 * FRAGS * 64;
     const int c = blockIdx.y, i = blockIdx.z, half = lane >> 5, n31 = lane & 31;
     const int g = blockIdx.x % a.c.Hkv;
@@ -730,7 +731,7 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 && !F32 ? 8 / WV : 1) void k_kv8_t
     const int full = a.t.pos[i] < 0 ? 0 : a.t.pos[i], len = full < a.max_len ? full : a.max_len;
     const int64_t at0 = (int64_t) full - r.all;
     const Kv8Seen first = kv8_seen(at0 + R0 / a.rep, len, a.window), last = kv8_seen(at0 + (R0 + nrow - 1) / a.rep, len, a.window);
-    const int64_t c0 = (int64_t) c * a.C, c1 = c0 + a.C;
+    const int64_t c0 = kv8_start(at0, len, a.window) + (int64_t) c * a.C, c1 = c0 + a.C;
     const int lo = first.lo > c0 ? first.lo : (int) (c0 < last.hi ? c0 : last.hi), hi = last.hi < c1 ? last.hi : (int) c1;
     if (a.nch > 1 && lo >= hi) return;
     const int pbeg = lo / KV8_PAGE, pend = (hi + KV8_PAGE - 1) / KV8_PAGE;
@@ -755,46 +756,49 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 && !F32 ? 8 / WV : 1) void k_kv8_t
             dst[u][1] = dst[u][0] + 128;
         }
     }
-    uint4 raw[NU];
-    auto load = [&](int id) {
-        const int8_t * p = a.c.codes + ((int64_t) id * a.c.Hkv + g) * 2 * KV8_PAGE * D;
+    uint4 raw[NU], piece;
+    auto load_unit = [&](int u, int64_t at) { raw[u] = *(const uint4 *) (a.c.codes + at + src[u]); };
+    auto load = [&](int64_t at) {
 #pragma unroll
-        for (int u = 0; u < NU; u++) raw[u] = *(const uint4 *) (p + src[u]);
+        for (int u = 0; u < NU; u++) load_unit(u, at);
+    };
+    auto store_piece = [&](int k, uint4 * to) {                  // a quarter of a unit: 4 codes of a lane
+        const int u = k >> 2, e = k & 3;
+        codes_f16(e == 0 ? raw[u].x : (e == 1 ? raw[u].y : (e == 2 ? raw[u].z : raw[u].w)), e & 1 ? piece.z : piece.x, e & 1 ? piece.w : piece.y);
+        if (e & 1) to[dst[u][e >> 1]] = piece;
     };
     auto store = [&](uint4 * to) {
 #pragma unroll
-        for (int u = 0; u < NU; u++) {
-            uint4 x, y;
-            codes_f16(raw[u].x, x.x, x.y);
-            codes_f16(raw[u].y, x.z, x.w);
-            codes_f16(raw[u].z, y.x, y.y);
-            codes_f16(raw[u].w, y.z, y.w);
-            to[dst[u][0]] = x;
-            to[dst[u][1]] = y;
-        }
+        for (int k = 0; k < 4 * NU; k++) store_piece(k, to);
     };
     // ids and scales of 64 pages at a time, a page a lane: no load to wait for in the loop
-    int lid = 0;
+    int64_t lat = 0;                          // where its codes begin
     float lsk = 0.f, lls = 0.f;               // K's scale, log2 of V's
     auto fetch = [&](int p0) {
         const int at = p0 + KS * lane, id = at < pend ? kv8_page(tab, at, a.t.P, a.c.pages) : -1;
         const float * p = a.c.scales + ((int64_t) (id < 0 ? 0 : id) * a.c.Hkv + g) * 2;
         const bool bad = id < 0 || full > a.max_len;
-        lid = id < 0 ? 0 : id;
+        lat = ((int64_t) (id < 0 ? 0 : id) * a.c.Hkv + g) * 2 * KV8_PAGE * D;
         lsk = bad ? nan : p[0];
         lls = bad ? nan : __builtin_amdgcn_logf(p[1] < 1e-36f ? 1e-36f : p[1]);
+    };
+    auto lane_at = [&](int n) {
+        return (int64_t) ((uint64_t) (uint32_t) __builtin_amdgcn_readlane((int) (lat >> 32), n) << 32 | (uint32_t) __builtin_amdgcn_readlane((int) lat, n));
     };
     auto lane_f = [&](float v, int n) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), n)); };
 
     const int p0 = pbeg + grp, np = pend > p0 ? (pend - p0 + KS - 1) / KS : 0, rounds = pend > pbeg ? (pend - pbeg + KS - 1) / KS : 0;
-    float sk = 0.f, ls = 0.f, skn = 0.f, lsn = 0.f;
+    float qk[3] = {0.f, 0.f, 0.f}, qs[3] = {0.f, 0.f, 0.f};      // scales of pages n .. n + 2
+    int64_t next = 0;                         // where page n + 2 is
     if (np > 0) {                             // (the first page's codes are on their way while q is prepared)
         fetch(p0);
-        load(__builtin_amdgcn_readlane(lid, 0));
-        sk = lane_f(lsk, 0);
-        ls = lane_f(lls, 0);
-        skn = lane_f(lsk, 1);
-        lsn = lane_f(lls, 1);
+        load(lane_at(0));
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            qk[k] = lane_f(lsk, k);
+            qs[k] = lane_f(lls, k);
+        }
+        next = lane_at(0);
     }
 
     // this lane's row
@@ -841,55 +845,77 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 && !F32 ? 8 / WV : 1) void k_kv8_t
     float m = -inf, l = 0.f;
     int eref = -1000, emax = -1000;                              // no page yet
 
+    auto buffer = [&](int n) { return page + (n & 1) * FRAGS * 64; };
     if (np > 0) {
         store(page);
-        load(__builtin_amdgcn_readlane(lid, np > 1 ? 1 : 0));
+        load(lane_at(np > 1 ? 1 : 0));
     }
-    for (int n = 0; n < rounds; n++) {
-        const int t0 = (p0 + n * KS) * KV8_PAGE, n2 = n + 2;
-        const uint4 * cur = page + (n & 1) * FRAGS * 64;
-        float skc = sk, lsc = ls;
-        if ((n2 & 63) == 0 && n2 < np) fetch(p0 + n2 * KS);
-        lds_barrier();                                           // cur is whole, the other buffer is read
-        const bool skip = !live || n >= np || t0 >= wlast.hi || t0 + KV8_PAGE <= wfirst.lo;
-        f32x16 sc[2];
-        f32x4 mk[2][4];
-        if (MASK && !skip) {                  // (ahead of the next page's loads, which would be waited for with it)
+    f32x16 sc[2];
+    f32x4 mk[2][4];
+    f16x2 p[PARTS][2][8];
+    // step k of the scores' products, of a page's K in LDS
+    const f32x16 zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+    auto k_step = [&](int k, uint4 fr) {
+#pragma unroll
+        for (int y = 0; y < PARTS; y++)
+            sc[k / NC] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, fr), q[y][k % NC], k % NC || y ? sc[k / NC] : zero, 0, 0, 0);
+    };
+    // ... and of o's, of V: 16 tokens (T, v), 32 d each
+    auto v_frag = [&](int k) { return 2 * NC + k % ND * 4 + k / ND; };
+    auto v_step = [&](int k, uint4 fr) {
+        const int T = k / ND >> 1, v = k / ND & 1, t = k % ND;
+#pragma unroll
+        for (int y = 0; y < PARTS; y++) {
+            f16x8 b;
+#pragma unroll
+            for (int e = 0; e < 8; e++) b[e] = p[y][T][2 * (v + 2 * (e >> 2)) + ((e & 3) >> 1)][e & 1];
+            o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, fr), b, o[t], 0, 0, 0);
+        }
+    };
+    // the scores of page n; between the products the codes that are in registers go to LDS as page n + 1, and the loads of
+    // those of page n + 2 are issued
+    auto scores = [&](int n) {
+        const int t0 = (p0 + n * KS) * KV8_PAGE;
+        const uint4 * cur = buffer(n);
+        uint4 * to = buffer(n + 1);
+        if (MASK) {                           // (ahead of the codes' loads, which would be waited for with it)
 #pragma unroll
             for (int T = 0; T < 2; T++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) mk[T][e] = mask4(a.mask + i * a.mld + t0, 32 * T + 8 * e + 4 * half, hi - t0);
         }
-        if (!skip) {
-            // fragments four products ahead of their use, held in this order (the scheduler would read each just before it)
-            uint4 fr[4];
+        // fragments four products ahead of their use, held in this order (the scheduler would read each just before it)
+        uint4 fr[4];
 #pragma unroll
-            for (int k = 0; k < 4; k++) fr[k] = cur[k * 64 + lane];
+        for (int k = 0; k < 4; k++) fr[k] = cur[k * 64 + lane];
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int T = 0; T < 2; T++)
+        for (int k = 0; k < 2 * NC; k++) {
+            k_step(k, fr[k & 3]);
+            if (k + 4 < 2 * NC) fr[k & 3] = cur[(k + 4) * 64 + lane];
 #pragma unroll
-                for (int e = 0; e < 16; e++) sc[T][e] = 0.f;
+            for (int e = k * 4 * NU / (2 * NC); e < (k + 1) * 4 * NU / (2 * NC); e++) {
+                store_piece(e, to);
+                if ((e & 3) == 3) load_unit(e >> 2, next);
+            }
             __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int k = 0; k < 2 * NC; k++) {
-#pragma unroll
-                for (int y = 0; y < PARTS; y++)
-                    sc[k / NC] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, fr[k & 3]), q[y][k % NC], sc[k / NC], 0, 0, 0);
-                if (k + 4 < 2 * NC) fr[k & 3] = cur[(k + 4) * 64 + lane];
-                __builtin_amdgcn_sched_barrier(0);
-            }
         }
-        if (n + 1 < np) {
-            store(page + (~n & 1) * FRAGS * 64);
-            sk = skn;
-            ls = lsn;
-            if (n2 < np) {
-                load(__builtin_amdgcn_readlane(lid, n2 & 63));
-                skn = lane_f(lsk, n2 & 63);
-                lsn = lane_f(lls, n2 & 63);
-            }
+    };
+    auto pass_on = [&](int n) {               // the codes alone
+        store(buffer(n + 1));
+        load(next);
+    };
+    auto look_up = [&](int n) {               // page n + 2 (past the last: it again, unused)
+        const int n2 = n + 2;
+        if (n2 < np) {
+            if ((n2 & 63) == 0) fetch(p0 + n2 * KS);
+            next = lane_at(n2 & 63);
+            qk[2] = lane_f(lsk, n2 & 63);
+            qs[2] = lane_f(lls, n2 & 63);
         }
-        if (skip) continue;
+    };
+    auto weights = [&](int n, float skc, float lsc) {
+        const int t0 = (p0 + n * KS) * KV8_PAGE;
         // a page of a NaN scale: rows that see it become NaN at its end; with the scale in their scores the others would, too
         const bool poison = !(lsc < 128.f) || skc != skc;
         if (skc != skc) skc = 1.f;
@@ -925,14 +951,14 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 && !F32 ? 8 / WV : 1) void k_kv8_t
         // V's scale as a power of two within 2^4 of the reference, which moves otherwise (never 2^60 below the largest)
         if (!(lsc < 128.f)) lsc = eref > -1000 ? (float) eref : 0.f;
         const float step = MASK ? 3.f / LOG2E : 3.f;
-        const bool move = mx > m + step || (m == -inf && mx > m);
-        const bool shift = fabsf(lsc - (float) eref) > 4.f;
-        if (__any(move) || shift) {
+        const bool move = mx > m + step;      // (m = -inf: any score)
+        const bool shift_v = fabsf(lsc - (float) eref) > 4.f;
+        if (__any(move) || shift_v) {
             const float mn = move ? mx : m, base = mn == -inf ? 0.f : mn;
             float f = m == -inf ? 0.f : __builtin_amdgcn_exp2f(MASK ? (m - base) * LOG2E : m - base);
             l *= f;
             m = mn;
-            if (shift) {
+            if (shift_v) {
                 int e = (int) rintf(lsc);
                 emax = e > emax ? e : emax;
                 e = e < emax - 60 ? emax - 60 : e;
@@ -962,7 +988,6 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 && !F32 ? 8 / WV : 1) void k_kv8_t
             k = 1.f;
             off = lr;
         }
-        f16x2 p[PARTS][2][8];
         float sum = 0.f;
         const f16x2 one = {(_Float16) 1.f, (_Float16) 1.f};
 #pragma unroll
@@ -982,22 +1007,29 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 && !F32 ? 8 / WV : 1) void k_kv8_t
             }
         l = fmaf(sum, __builtin_amdgcn_exp2f(-lr), l);
         if (poison && mine.lo < t0 + KV8_PAGE && mine.hi > t0) l = nan;
+    };
+    auto values = [&](int n) {
+        const uint4 * cur = buffer(n);
 #pragma unroll
-        for (int T = 0; T < 2; T++)
+        for (int k = 0; k < 2 * NC; k++) v_step(k, cur[v_frag(k) * 64 + lane]);
+    };
+    auto shift = [&] {
 #pragma unroll
-            for (int v = 0; v < 2; v++) {
-                f16x8 b[PARTS];
-#pragma unroll
-                for (int y = 0; y < PARTS; y++)
-#pragma unroll
-                    for (int e = 0; e < 8; e++) b[y][e] = p[y][T][2 * (v + 2 * (e >> 2)) + ((e & 3) >> 1)][e & 1];
-#pragma unroll
-                for (int t = 0; t < ND; t++) {
-                    const f16x8 c = __builtin_bit_cast(f16x8, cur[(2 * NC + t * 4 + T * 2 + v) * 64 + lane]);
-#pragma unroll
-                    for (int y = 0; y < PARTS; y++) o[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(c, b[y], o[t], 0, 0, 0);
-                }
-            }
+        for (int k = 0; k < 2; k++) {
+            qk[k] = qk[k + 1];
+            qs[k] = qs[k + 1];
+        }
+    };
+    for (int n = 0; n < rounds; n++) {
+        look_up(n);
+        lds_barrier();                        // page n is whole, the other buffer is read
+        const int t0 = (p0 + n * KS) * KV8_PAGE;
+        if (live && n < np && t0 < wlast.hi && t0 + KV8_PAGE > wfirst.lo) {
+            scores(n);
+            weights(n, qk[0], qs[0]);
+            values(n);
+        } else pass_on(n);
+        shift();
     }
     if (KS > 1) {                             // the groups meet in the first, through LDS, in units of 2^m and 2^eref
         lds_barrier();
@@ -1081,7 +1113,8 @@ __global__ __launch_bounds__(KT) void k_kv8_combine(Kv8AttnArgs a) {
     if (W == 1 ? !live : (blockIdx.x * (CW / W)) / a.Hq >= r.n) return;       // (W > 1 meets at a barrier: leave together)
     const int full = a.t.pos[i] < 0 ? 0 : a.t.pos[i], len = full < a.max_len ? full : a.max_len;
     const Kv8Seen s = kv8_seen((int64_t) full - r.all + j, len, a.window);
-    const int ca = s.lo / a.C, cb = live && s.hi > s.lo ? (s.hi - 1) / a.C + 1 : ca;         // the chunks that this row sees
+    const int at = kv8_start((int64_t) full - r.all, len, a.window);
+    const int ca = (s.lo - at) / a.C, cb = live && s.hi > s.lo ? (s.hi - 1 - at) / a.C + 1 : ca;             // the chunks that this row sees
     const int64_t o = (r.row + (live ? j : 0)) * a.Hq + h;
     const float * wo = a.ws + o * a.nch * D, * wml = a.ws + a.t.T * a.Hq * a.nch * D + o * a.nch * 2;
     // (maxima are in powers of 2 without a mask, in powers of e with one: its lowest value has to fit)
@@ -1133,7 +1166,8 @@ __global__ __launch_bounds__(KT) void k_kv8_join(Kv8AttnArgs a) {
     if (j >= r.n) return;
     const int full = a.t.pos[i] < 0 ? 0 : a.t.pos[i], len = full < a.max_len ? full : a.max_len;
     const Kv8Seen s = kv8_seen((int64_t) full - r.all + j, len, a.window);
-    const int ca = s.lo / a.C, n = s.hi > s.lo ? (s.hi - 1) / a.C + 1 - ca : 0;         // the chunks that this row sees
+    const int at = kv8_start((int64_t) full - r.all, len, a.window);
+    const int ca = (s.lo - at) / a.C, n = s.hi > s.lo ? (s.hi - 1 - at) / a.C + 1 - ca : 0;        // the chunks that this row sees
     const int64_t o = (r.row + j) * a.Hq + h;
     const float * wo = a.ws + (o * a.nch + ca) * D + d, * wml = a.ws + a.t.T * a.Hq * a.nch * D + (o * a.nch + ca) * 2;
     const float unit = a.mask ? LOG2E : 1.f, sink = a.sinks ? a.sinks[h] * (a.mask ? 1.f : LOG2E) : -__builtin_inff();
@@ -1178,10 +1212,12 @@ AttnPlan attn_plan(int f32, int Hq, int D, int Hkv, int nseq, int max_n, int max
     // (8 waves need whole units of a page: D up to 64 and from 97 to 128.)
     const bool eight = !f32 && (D <= 64 || (D > 96 && D <= 128));
     p.wv = eight && (rows <= 128 || (int64_t) max_n * 4 <= max_len) ? 8 : 4;
-    p.ks = p.wv == 8 && rows <= 128 ? 2 : 1;
+    const bool two = eight && (rows <= 128 || ((int64_t) max_n * 4 > max_len && (rows + 127) / 128 * Hkv * nseq <= 256));
+    if (two) p.wv = 8;
+    p.ks = two ? 2 : 1;
     const int group = p.tile ? 32 * p.wv / p.ks : 4 * p.RS;
     p.ngrp = (int) ((rows + group - 1) / group);
-    const int64_t wgs = (int64_t) Hkv * p.ngrp * nseq, eff = window > 0 && window + max_n < max_len ? window + max_n : max_len;
+    const int64_t wgs = (int64_t) Hkv * p.ngrp * nseq, eff = window > 0 ? std::min<int64_t>(max_len, (int64_t) window + max_n + KV8_PAGE - 2) : max_len;
     int64_t C;
     if (p.tile) {
         // Split along the tokens where the workgroups leave CUs without, in chunks of 512 tokens or more (2048 for a twofold
@@ -1189,17 +1225,17 @@ AttnPlan attn_plan(int f32, int Hq, int D, int Hkv, int nseq, int max_n, int max
         // and further where whole rounds of the workgroups come out fuller.
         const int64_t slots = p.wv == 8 || D > 128 || f32 ? 256 : 512;
         auto used = [&](int64_t n) { return (double) (wgs * n) / (double) ((wgs * n + slots - 1) / slots * slots); };
-        int64_t nch = std::min<int64_t>(std::max<int64_t>(slots / wgs, 1), (max_len + 511) / 512);
-        if (nch == 2 && max_len < 4096) nch = 1;
+        int64_t nch = std::min<int64_t>(std::max<int64_t>(slots / wgs, 1), (eff + 511) / 512);
+        if (nch == 2 && eff < 4096) nch = 1;
         if ((int64_t) max_n * 4 <= max_len)
-            for (int64_t n = nch + 1; n <= 8 && max_len / n >= 2048; n++)
+            for (int64_t n = nch + 1; n <= 8 && eff / n >= 2048; n++)
                 if (used(n) > 1.15 * used(nch)) nch = n;
-        C = ((max_len + nch - 1) / nch + KV8_PAGE - 1) / KV8_PAGE * KV8_PAGE;
+        C = ((eff + nch - 1) / nch + KV8_PAGE - 1) / KV8_PAGE * KV8_PAGE;
     } else {
         const int64_t single = 2048;
-        C = eff <= single ? max_len : std::min<int64_t>(std::max<int64_t>(eff * wgs / 512, 512), 2048);
+        C = eff <= single ? eff : std::min<int64_t>(std::max<int64_t>(eff * wgs / 512, 512), 2048);
         // eight waves a workgroup where the workgroups leave CUs without
-        p.sw = wgs * ((max_len + C - 1) / C) <= 256 && D <= 128 ? 8 : 4;
+        p.sw = wgs * ((eff + C - 1) / C) <= 256 && D <= 128 ? 8 : 4;
         // non-temporal loads where the codes are more than the caches would keep for another call (MB, us without -> with: 1070
         // 187 -> 170, 578 116 -> 103, 245 64 -> 57, 134 27.4 -> 24.1, 67 15.3 -> 15.4, 33 13.6 -> 15.8, 4 11.0 -> 13.6)
         p.nt = p.ngrp == 1 && 2 * eff * nseq * Hkv * D >= 100000000;
@@ -1207,7 +1243,7 @@ AttnPlan attn_plan(int f32, int Hq, int D, int Hkv, int nseq, int max_n, int max
         C = (C + round - 1) / round * round;
     }
     p.C = (int) (C > (1 << 30) ? 1 << 30 : C);
-    p.nch = (int) ((max_len + (int64_t) p.C - 1) / p.C);
+    p.nch = (int) ((eff + (int64_t) p.C - 1) / p.C);
     p.fold = p.wv == 4 && wgs * p.nch <= 512;
     return p;
 }
