@@ -713,11 +713,12 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 && !F32 ? 8 / WV : 1) void k_kv8_t
     constexpr int WR = WV / KS, TR = 32 * WR, NU = 2 * NC / WR, ND = NC / 2;         // waves over the rows, rows, a wave's load
     constexpr int FRAGS = 4 * NC;                                                    // units, d tiles of 32, KiB of a page
     static_assert(NU * WR == 2 * NC, "the waves share a page's units evenly");
-    extern __shared__ __align__(16) uint4 lds4[];                // [KS][2][FRAGS][64]
+    extern __shared__ __align__(16) uint4 lds4[];                // [KS][2][FRAGS][64], MASK: [KS][2][64] floats
     const int D = a.c.D, nc = D / 16, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // of KS groups of waves, each with every KS-th page; waves 4 apart share a SIMD: the first 64 rows' are on all four
     const int grp = wave / WR, w = (wave % WR) ^ (2 * grp);
     uint4 * page = lds4 + grp * 2 * FRAGS * 64;
+    float * masks = (float *) (lds4 + KS * 2 * FRAGS * 64) + grp * 2 * KV8_PAGE;                 // the pages' mask values
     const int c = blockIdx.y, i = blockIdx.z, half = lane >> 5, n31 = lane & 31;
     const int g = blockIdx.x % a.c.Hkv;
     int z = blockIdx.x / a.c.Hkv;
@@ -762,6 +763,11 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 && !F32 ? 8 / WV : 1) void k_kv8_t
 #pragma unroll
         for (int u = 0; u < NU; u++) load_unit(u, at);
     };
+    float mraw = 0.f;                         // the mask of the page in registers, a token a lane
+    auto load_mask = [&](int pg) {
+        const int64_t at = (int64_t) pg * KV8_PAGE + lane;
+        if (MASK) mraw = at < hi ? a.mask[i * a.mld + at] : 0.f;
+    };
     auto store_piece = [&](int k, uint4 * to) {                  // a quarter of a unit: 4 codes of a lane
         const int u = k >> 2, e = k & 3;
         codes_f16(e == 0 ? raw[u].x : (e == 1 ? raw[u].y : (e == 2 ? raw[u].z : raw[u].w)), e & 1 ? piece.z : piece.x, e & 1 ? piece.w : piece.y);
@@ -793,6 +799,7 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 && !F32 ? 8 / WV : 1) void k_kv8_t
     if (np > 0) {                             // (the first page's codes are on their way while q is prepared)
         fetch(p0);
         load(lane_at(0));
+        load_mask(p0);
 #pragma unroll
         for (int k = 0; k < 2; k++) {
             qk[k] = lane_f(lsk, k);
@@ -848,10 +855,11 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 && !F32 ? 8 / WV : 1) void k_kv8_t
     auto buffer = [&](int n) { return page + (n & 1) * FRAGS * 64; };
     if (np > 0) {
         store(page);
+        if (MASK) masks[lane] = mraw;
         load(lane_at(np > 1 ? 1 : 0));
+        load_mask(p0 + KS);
     }
     f32x16 sc[2];
-    f32x4 mk[2][4];
     f16x2 p[PARTS][2][8];
     // step k of the scores' products, of a page's K in LDS
     const f32x16 zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
@@ -875,15 +883,9 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 && !F32 ? 8 / WV : 1) void k_kv8_t
     // the scores of page n; between the products the codes that are in registers go to LDS as page n + 1, and the loads of
     // those of page n + 2 are issued
     auto scores = [&](int n) {
-        const int t0 = (p0 + n * KS) * KV8_PAGE;
         const uint4 * cur = buffer(n);
         uint4 * to = buffer(n + 1);
-        if (MASK) {                           // (ahead of the codes' loads, which would be waited for with it)
-#pragma unroll
-            for (int T = 0; T < 2; T++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) mk[T][e] = mask4(a.mask + i * a.mld + t0, 32 * T + 8 * e + 4 * half, hi - t0);
-        }
+        if (MASK) masks[(~n & 1) * KV8_PAGE + lane] = mraw;
         // fragments four products ahead of their use, held in this order (the scheduler would read each just before it)
         uint4 fr[4];
 #pragma unroll
@@ -900,10 +902,13 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 && !F32 ? 8 / WV : 1) void k_kv8_t
             }
             __builtin_amdgcn_sched_barrier(0);
         }
+        load_mask(p0 + (n + 2) * KS);
     };
     auto pass_on = [&](int n) {               // the codes alone
         store(buffer(n + 1));
         load(next);
+        if (MASK) masks[(~n & 1) * KV8_PAGE + lane] = mraw;
+        load_mask(p0 + (n + 2) * KS);
     };
     auto look_up = [&](int n) {               // page n + 2 (past the last: it again, unused)
         const int n2 = n + 2;
@@ -925,7 +930,11 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 && !F32 ? 8 / WV : 1) void k_kv8_t
 #pragma unroll
             for (int T = 0; T < 2; T++)
 #pragma unroll
-                for (int e = 0; e < 16; e++) sc[T][e] = fmaf(sc[T][e], cs, mk[T][e >> 2][e & 3]);
+                for (int e = 0; e < 4; e++) {
+                    const f32x4 mk = *(const f32x4 *) (masks + (n & 1) * KV8_PAGE + 32 * T + 8 * e + 4 * half);
+#pragma unroll
+                    for (int v = 0; v < 4; v++) sc[T][4 * e + v] = fmaf(sc[T][4 * e + v], cs, mk[v]);
+                }
         }
         if (edge) {
             const int l0 = (mine.lo > lo ? mine.lo : lo) - t0 - 4 * half, h0 = (mine.hi < hi ? mine.hi : hi) - t0 - 4 * half;
@@ -1266,7 +1275,7 @@ template <int NC> hipError_t run_attn(const Kv8AttnArgs & a, const AttnPlan & p,
         return p.RS == 1 ? run_step<NC, 1, 4>(a, p, s) : run_step<NC, 2, 4>(a, p, s);
     }
     const dim3 grid((unsigned) (a.c.Hkv * p.ngrp), (unsigned) p.nch, (unsigned) a.t.nseq);
-    const size_t lds = 2 * 4 * NC * 1024;
+    const size_t lds = 2 * 4 * NC * 1024 + (a.mask ? 2 * KV8_PAGE * sizeof(float) : 0);
     if constexpr (NC <= 8 && NC % 4 == 0)
         if (p.wv == 8) {
             if (p.ks == 2 && a.mask) k_kv8_tile<NC, 8, 2, true, false><<<grid, 512, 2 * lds, s>>>(a);

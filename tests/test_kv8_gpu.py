@@ -328,6 +328,46 @@ def test_attn_long(gpu, dt, Hq, Hkv, D, S, window):
 
 
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("Hq,Hkv,D,n", [(8, 2, 128, 1), (4, 2, 64, 3), (8, 2, 128, 12), (4, 1, 256, 40), (6, 3, 96, 70), (2, 2, 64, 300)])
+def test_attn_windows_of_several_chunks(gpu, dt, Hq, Hkv, D, n):
+    """windows that are split over workgroups, beginning anywhere in a page and in any place of the sequence,
+    beside sequences shorter than the window"""
+    rng = np.random.default_rng(D + n)
+    lens = [9001, 2564 + n, 70 + n, 5555, n, 6016]
+    print(f"kv8_attn window chunks {dt} {Hq}/{Hkv}/{D} n={n}", flush=True)
+    for window in (2500, 4097):
+        _close(*_attn_case(rng, dt, Hq, Hkv, D, lens, [n, 1, n, 2, n, 1], window=window, sinks=window == 2500))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("D", [64, 80, 128])
+@pytest.mark.parametrize("masked", [False, True])
+def test_attn_prompts_of_many_workgroups(gpu, dt, D, masked):
+    """more prompts than the card runs at once, on themselves and behind a few tokens"""
+    rng = np.random.default_rng(D)
+    n = [130, 129, 1, 77, 130, 128, 64, 130, 33]
+    print(f"kv8_attn many prompts {dt} D={D} masked={masked}", flush=True)
+
+    def mask(m):
+        m[2, :64] = -np.inf
+        m[4, 100:] = -np.inf
+    _close(*_attn_case(rng, dt, 32, 16, D, [k + 9 * i for i, k in enumerate(n)], n, mask=mask if masked else None))
+
+
+@pytest.mark.parametrize("dt,D,n,masked", [("bf16", 64, 20, False), ("bf16", 128, 20, True), ("bf16", 128, 130, False),
+                                           ("f32", 96, 70, False), ("f32", 128, 20, True)])
+def test_attn_many_pages_of_one_workgroup(gpu, dt, D, n, masked):
+    """so many sequences and heads that none is split, one of them of 150 pages, masked in places"""
+    rng = np.random.default_rng(D + n)
+    lens = [9601] + [n + 40 * i for i in range(15)]
+    print(f"kv8_attn many pages {dt} D={D} n={n} masked={masked}", flush=True)
+
+    def mask(m):
+        m[0, 3000:7000] = -np.inf
+    _close(*_attn_case(rng, dt, 16, 16, D, lens, [n] + [3] * 14 + [n], mask=mask if masked else None))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
 @pytest.mark.parametrize("n", [1, 5, 150])
 @pytest.mark.parametrize("sinks", [False, True])
 def test_attn_masks(gpu, dt, n, sinks):
