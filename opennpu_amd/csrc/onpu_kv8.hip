@@ -61,16 +61,24 @@ __device__ __forceinline__ int quant(float x, float s, float inv) {
     if (e < -h || (e == -h && odd)) c -= 1.f;
     return (int) fminf(fmaxf(c, -127.f), 127.f);
 }
-// the codes of four values, their lowest bytes: x / s + 1.5 2^23 in one fma is the nearest integer (ties to even) of
-// x * (1 / s) in the sum's last bits, right unless the remainder x - c s is within 2^-16 s of s / 2, which `far` (the
-// largest |x - c s| so far) tells: then quant decides
-__device__ __forceinline__ uint32_t near4(const float (&x)[4], float s, float inv, float & far) {
+// The codes of four values, their lowest bytes: c = x / s + 1.5 2^23 in one fma has the nearest integer of x * (1 / s) in
+// its last bits, right unless x - c s is all but s / 2. For fp32 `far`, the largest |x - c s| so far, tells (within
+// 2^-16 s of s / 2, three values of 10^5): then quant decides. bf16 values of a page whose largest is bf16 as well fall
+// there in almost every wave, so each is put right at once by comparing with s / 2, and far is s / 2 after an exact tie.
+// (8192 tokens x 8 x 128 bf16, K and V: 19.5 us with far alone, 17.8 with this.)
+template <bool F32> __device__ __forceinline__ uint32_t near4(const float (&x)[4], float s, float inv, float & far) {
     uint32_t y[4];
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-        const float c = fmaf(x[e], inv, 12582912.f);
-        far = fmaxf(far, fabsf(fmaf(-(c - 12582912.f), s, x[e])));
-        y[e] = __float_as_uint(c);
+        const float c = fmaf(x[e], inv, 12582912.f), r = fmaf(-(c - 12582912.f), s, x[e]);
+        if (F32) {
+            far = fmaxf(far, fabsf(r));
+            y[e] = __float_as_uint(c);
+        } else {
+            const float h = 0.5f * s;
+            far = fabsf(r) == h ? h : far;
+            y[e] = __float_as_uint(fabsf(r) > h ? c + copysignf(1.f, r) : c);
+        }
     }
     return __builtin_amdgcn_perm(y[1], y[0], 0x0c0c0400u) | __builtin_amdgcn_perm(y[3], y[2], 0x04000c0cu);
 }
@@ -223,7 +231,7 @@ __global__ __launch_bounds__(KT) void k_kv8_write(WriteArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             const float x[4] = {raw_at<F32>(xk[k], 4 * e), raw_at<F32>(xk[k], 4 * e + 1), raw_at<F32>(xk[k], 4 * e + 2), raw_at<F32>(xk[k], 4 * e + 3)};
-            y[e] = near4(x, s[0], inv[0], far);
+            y[e] = near4<F32>(x, s[0], inv[0], far);
         }
         if (far > lim[0])
 #pragma unroll
@@ -249,7 +257,7 @@ __global__ __launch_bounds__(KT) void k_kv8_write(WriteArgs a) {
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const float x[4] = {raw_at<F32>(xv[k][0], e), raw_at<F32>(xv[k][1], e), raw_at<F32>(xv[k][2], e), raw_at<F32>(xv[k][3], e)};
-            y[e] = near4(x, s[1], inv[1], far);
+            y[e] = near4<F32>(x, s[1], inv[1], far);
         }
         if (far > lim[1])
 #pragma unroll

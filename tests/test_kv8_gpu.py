@@ -123,6 +123,26 @@ def test_write_borders_between_codes(gpu):
         assert np.array_equal(gc.cpu().numpy(), ref.codes), amax
 
 
+def test_write_bf16_ties_and_near_ties(gpu):
+    """the bf16 values below a page's largest, down to its 2^-9: a scale of few bits makes exact ties of many, any
+    other quotients within a rounding of one"""
+    import torch
+    from opennpu_amd.device import kv8_write
+    D, n = 128, 64
+    codes, scales = np.zeros((2, 1, 2, 64 * D), np.int8), np.zeros((2, 1, 2), np.float32)
+    gc, gs, ref = _dev(codes), _dev(scales), Cache(codes, scales)
+    for bits in [0x42fe, 0x3f80, 0x3fc8, 0x4049, 0x0301, 0x7f7f] + list(range(0x4080, 0x4100, 5)):
+        top = np.arange(max(bits - 9 * 128, 0), bits + 1, dtype=np.uint32)
+        x = np.concatenate([top << 16, (top << 16) | np.uint32(1 << 31)]).view(np.float32)
+        x = np.resize(x, (n, 1, D))
+        t = _dev(x).to(torch.bfloat16)
+        assert np.array_equal(t.float().cpu().numpy(), x)
+        kv8_write(gc, gs, t, t.flip(0), _i32([[1]]), _i32([0]))
+        ref.write(x.astype(np.float64), x[::-1].astype(np.float64), [1], 0)
+        assert np.array_equal(gs.cpu().numpy(), ref.scales)
+        assert np.array_equal(gc.cpu().numpy(), ref.codes), hex(bits)
+
+
 def test_write_values_that_are_not_finite(gpu):
     """the page, head and K | V that got one reads as NaN, nothing else does; beginning the page anew clears it"""
     import torch
