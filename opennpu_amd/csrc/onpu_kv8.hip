@@ -45,6 +45,9 @@ template <bool F32> __device__ __forceinline__ void load16(const void * base, in
 // and stays in registers across the maximum (a lane has 16 d of a K token and 8 d of 4 V tokens, so that
 // V's bytes of 4 tokens are whole words); K's codes go out from there, V's through LDS in the page's
 // order. A page with earlier tokens is changed in place, its new bytes alone unless the scale grows.
+// 8192 tokens x 8 x 128 bf16: 17.0 us for 50 MB, 3.0 TB/s (all pages are on the card at once, so the loads, the
+// codes' arithmetic and the stores follow one another: 44 % of the waves' cycles wait); one token: 4.4 us, the latency
+// of position, table, scale and row in turn.
 struct WriteArgs {
     Kv8Cache c;
     Kv8Table t;
@@ -89,11 +92,16 @@ template <bool F32> __device__ __forceinline__ uint32_t raw_max(uint32_t m, uint
 #pragma unroll
     for (int e = 0; e < 4; e++)
         m = F32 ? max(m, w[e] & 0x7fffffffu)
-                : __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, m), __builtin_bit_cast(u16x2, w[e] & 0x7fff7fffu)));
+                : __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, m),
+                                                                         __builtin_bit_cast(u16x2, w[e] & 0x7fff7fffu)));
     return m;
 }
 __device__ __forceinline__ uint32_t bytes4(int a, int b, int c, int d) {
     return (uint32_t) (a & 255) | (uint32_t) (b & 255) << 8 | (uint32_t) (c & 255) << 16 | (uint32_t) d << 24;
+}
+
+template <bool F32> __device__ __forceinline__ float one_at(const void * x, int64_t at) {
+    return F32 ? ((const float *) x)[at] : bf16_to_f32(((const uint16_t *) x)[at]);
 }
 
 // the scale of values whose largest magnitude has these bits
@@ -101,11 +109,16 @@ __device__ __forceinline__ float scale_for(uint32_t bits) {
     return bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(__uint_as_float(bits), KV8_TINY) / 127.f;
 }
 
+// Where word w of V's codes is in LDS: a lane turns the 8 words of 8 d, lanes differ in 16 d and in the token's quad,
+// which are 256 and 64 words apart; 4 words between every 64 leave 16 banks of 64 to them instead of 2
+// (8192 tokens x 8 x 128 bf16 written in 17.0 us, read in 10.9; without 17.8, 11.9).
+__device__ __forceinline__ int vt_at(int w) { return w + (w >> 6) * 4; }
+
 // NQ: D up to 128 NQ
 template <bool F32, int NQ>
 __global__ __launch_bounds__(KT) void k_kv8_write(WriteArgs a) {
     constexpr int NK = 2 * NQ, NV = NQ;       // units of a lane: 16 d of one K token, 8 d of 4 V tokens
-    extern __shared__ __align__(16) uint32_t vt[];               // V's 64 D codes
+    extern __shared__ __align__(16) uint32_t vt[];               // V's 64 D codes (vt_at)
     __shared__ uint32_t wmax[2][KT / 64];
     const int D = a.c.D, NC = D / 16, t = threadIdx.x, g = blockIdx.x % a.c.Hkv, w = blockIdx.x / a.c.Hkv, i = blockIdx.y;
     const Kv8Rows r = kv8_rows(a.t.off, i, a.t.T, a.t.max_n);
@@ -126,7 +139,7 @@ __global__ __launch_bounds__(KT) void k_kv8_write(WriteArgs a) {
         for (int kv = 0; kv < 2; kv++)
             for (int u = t; u < (s1 - s0) * D; u += KT) {
                 const int64_t at = (row0 + s0 + u / D) * a.rs[kv] + g * a.hs[kv] + u % D;
-                m[kv] = max(m[kv], (F32 ? ((const uint32_t *) a.x[kv])[at] : (uint32_t) ((const uint16_t *) a.x[kv])[at] << 16) & 0x7fffffffu);
+                m[kv] = max(m[kv], __float_as_uint(fabsf(one_at<F32>(a.x[kv], at))));
             }
     } else {
 #pragma unroll
@@ -193,7 +206,7 @@ __global__ __launch_bounds__(KT) void k_kv8_write(WriteArgs a) {
             for (int u = t; u < (s1 - s0) * D; u += KT) {
                 const int tok = s0 + u / D, d = u % D;
                 const int64_t at = (row0 + tok) * a.rs[kv] + g * a.hs[kv] + d;
-                const float x = F32 ? ((const float *) a.x[kv])[at] : bf16_to_f32(((const uint16_t *) a.x[kv])[at]);
+                const float x = one_at<F32>(a.x[kv], at);
                 out[kv ? KV8_PAGE * D + kv8_v_at(D, tok, d) : kv8_k_at(D, tok, d)] = (int8_t) quant(x, s[kv], inv[kv]);
             }
         return;
@@ -206,7 +219,7 @@ __global__ __launch_bounds__(KT) void k_kv8_write(WriteArgs a) {
                 int q[4];
                 for (int e = 0; e < 4; e++) {
                     const int64_t at = (row0 + tok) * a.rs[0] + g * a.hs[0] + d + e;
-                    q[e] = quant(F32 ? ((const float *) a.x[0])[at] : bf16_to_f32(((const uint16_t *) a.x[0])[at]), s[0], inv[0]);
+                    q[e] = quant(one_at<F32>(a.x[0], at), s[0], inv[0]);
                 }
                 y = bytes4(q[0], q[1], q[2], q[3]);
             }
@@ -216,7 +229,7 @@ __global__ __launch_bounds__(KT) void k_kv8_write(WriteArgs a) {
             for (int e = 0; e < 4; e++)
                 if (4 * vq + e < s1) {
                     const int64_t at = (row0 + 4 * vq + e) * a.rs[1] + g * a.hs[1] + vd;
-                    y |= (uint32_t) (quant(F32 ? ((const float *) a.x[1])[at] : bf16_to_f32(((const uint16_t *) a.x[1])[at]), s[1], inv[1]) & 255) << (8 * e);
+                    y |= (uint32_t) (quant(one_at<F32>(a.x[1], at), s[1], inv[1]) & 255) << (8 * e);
                 }
             *(uint32_t *) (out + KV8_PAGE * D + kv8_v_at(D, 4 * vq, vd)) = y;
         }
@@ -230,7 +243,8 @@ __global__ __launch_bounds__(KT) void k_kv8_write(WriteArgs a) {
         float far = 0.f;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const float x[4] = {raw_at<F32>(xk[k], 4 * e), raw_at<F32>(xk[k], 4 * e + 1), raw_at<F32>(xk[k], 4 * e + 2), raw_at<F32>(xk[k], 4 * e + 3)};
+            const float x[4] = {raw_at<F32>(xk[k], 4 * e), raw_at<F32>(xk[k], 4 * e + 1), raw_at<F32>(xk[k], 4 * e + 2),
+                                raw_at<F32>(xk[k], 4 * e + 3)};
             y[e] = near4<F32>(x, s[0], inv[0], far);
         }
         if (far > lim[0])
@@ -256,7 +270,8 @@ __global__ __launch_bounds__(KT) void k_kv8_write(WriteArgs a) {
         float far = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            const float x[4] = {raw_at<F32>(xv[k][0], e), raw_at<F32>(xv[k][1], e), raw_at<F32>(xv[k][2], e), raw_at<F32>(xv[k][3], e)};
+            const float x[4] = {raw_at<F32>(xv[k][0], e), raw_at<F32>(xv[k][1], e), raw_at<F32>(xv[k][2], e),
+                                raw_at<F32>(xv[k][3], e)};
             y[e] = near4<F32>(x, s[1], inv[1], far);
         }
         if (far > lim[1])
@@ -268,19 +283,20 @@ __global__ __launch_bounds__(KT) void k_kv8_write(WriteArgs a) {
         for (int e = 0; e < 8; e++) {
             const int at = kv8_v_at(D, 4 * q, d + e);
             if (merge) *(uint32_t *) (ov + at) = (y[e] & ~keep) | (keep ? *(uint32_t *) (ov + at) & keep : 0);
-            else vt[at / 4] = y[e] & ~keep;
+            else vt[vt_at(at / 4)] = y[e] & ~keep;
         }
     }
     if (merge) return;
     __syncthreads();
-    for (int u = t; u < 4 * D; u += KT) ((uint4 *) ov)[u] = ((const uint4 *) vt)[u];
+    for (int u = t; u < 4 * D; u += KT) ((uint4 *) ov)[u] = *(const uint4 *) (vt + vt_at(4 * u));
 }
 
 // ------------------------------------------------------------------ read
 // A workgroup per (page, kv head, sequence): value = code * scale, rounded once (bf16: that rounded
 // again); code + 128 by an unsigned byte's conversion, less 128 in the product's fma, whose one rounding is
 // the product's. A page that the table does not have reads as NaN. Bound by the bytes: a lane writes 16 d
-// of a K token and 8 d of 4 V tokens, V's words turned through LDS.
+// of a K token and 8 d of 4 V tokens, V's words turned through LDS. 8192 tokens x 8 x 128 to bf16: 10.9 us for 50 MB,
+// 4.6 TB/s.
 struct ReadArgs {
     Kv8Cache c;
     Kv8Table t;
@@ -310,7 +326,7 @@ template <bool F32, int N> __device__ __forceinline__ void put(void * y, int64_t
 
 template <bool F32>
 __global__ __launch_bounds__(KT) void k_kv8_read(ReadArgs a) {
-    extern __shared__ __align__(16) uint32_t vt[];               // V's 64 D codes
+    extern __shared__ __align__(16) uint32_t vt[];               // V's 64 D codes (vt_at)
     const int D = a.c.D, NC = D / 16, t = threadIdx.x, g = blockIdx.x % a.c.Hkv, w = blockIdx.x / a.c.Hkv, i = blockIdx.y;
     const Kv8Rows r = kv8_rows(a.t.off, i, a.t.T, a.t.max_n);
     const int64_t p0 = a.t.pos[i], pg = (p0 - (p0 & (KV8_PAGE - 1))) / KV8_PAGE + w, base = pg * KV8_PAGE;
@@ -320,7 +336,7 @@ __global__ __launch_bounds__(KT) void k_kv8_read(ReadArgs a) {
     const int64_t row0 = r.row + (base - p0);
     const int8_t * in = a.c.codes + ((int64_t) (id < 0 ? 0 : id) * a.c.Hkv + g) * 2 * KV8_PAGE * D;
     const float * sc = a.c.scales + ((int64_t) (id < 0 ? 0 : id) * a.c.Hkv + g) * 2;
-    for (int u = t; u < 4 * D; u += KT) ((uint4 *) vt)[u] = ((const uint4 *) (in + KV8_PAGE * D))[u];
+    for (int u = t; u < 4 * D; u += KT) *(uint4 *) (vt + vt_at(4 * u)) = ((const uint4 *) (in + KV8_PAGE * D))[u];
     const float nan = __uint_as_float(0x7fc00000u), sk = id < 0 ? nan : sc[0], sv = id < 0 ? nan : sc[1];
     for (int u = s0 * NC + t; u < s1 * NC; u += KT) {
         const int tok = u / NC, d = u % NC * 16;
@@ -336,7 +352,7 @@ __global__ __launch_bounds__(KT) void k_kv8_read(ReadArgs a) {
         const int q = u / (2 * NC), d = u % (2 * NC) * 8;
         uint32_t x[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = vt[kv8_v_at(D, 4 * q, d + e) / 4] ^ 0x80808080u;
+        for (int e = 0; e < 8; e++) x[e] = vt[vt_at(kv8_v_at(D, 4 * q, d + e) / 4)] ^ 0x80808080u;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             if (4 * q + k < s0 || 4 * q + k >= s1) continue;
@@ -416,11 +432,16 @@ __device__ __forceinline__ float quad_sum(float x) {
 // fp32's own), in four signed bytes; the four are rows 4 h + part of a 16-row operand that holds 4 heads, their
 // integer sums exact. The scores come out as lane (row 4 h + part, quad), token 16 a + 4 quad + c: the
 // order of V's bytes, so the lane's weights, cut the same way (weight e^(x - m) <= 1 to 2^-31), are the other
-// product's operand without a move across lanes. A wave takes every fourth page, K of its next one loading
-// once this one's scores are out, V after its products; waves meet in LDS, chunks in k_kv8_combine.
-// RS sets of 4 rows; NC: chunks of 16 d (D / 16 or more).
+// product's operand without a move across lanes. A wave takes every SW-th page, K of its next one loading
+// once this one's scores are out, V after its products; waves meet in LDS, chunks in k_kv8_join or k_kv8_combine.
+// RS sets of 4 rows; NC: chunks of 16 d (D / 16 or more); NT: non-temporal loads of the codes.
+// 32 / 8 heads of 128: 65536 tokens 24.7 us (134 MB, 5.4 TB/s); 64 sequences of up to 8192 107 us (578 MB, 5.4 TB/s
+// of the 7.07 that streaming reads reach; FETCH_SIZE 1.014 times the codes). 200 tokens 6.2 us, the latency of lens,
+// table and codes in turn and the waves' joint. 64 / 8 heads of 64, a window of 4000 of 16 sequences: 17.8 us
+// (66 MB, 3.7 TB/s: two sets' cuts and softmax on half the bytes a page).
 template <int NC, int RS, int SW, bool MASK, bool NT>
-__global__ __launch_bounds__(64 * SW, SW == 8 ? 2 : (RS == 1 ? (NC <= 4 ? 4 : (NC <= 8 ? 3 : (NC <= 12 ? 2 : 1))) : (RS * NC <= 16 ? 2 : 1))) void k_kv8_step(Kv8AttnArgs a) {
+__global__ __launch_bounds__(64 * SW, SW == 8 ? 2 : (RS == 1 ? (NC <= 4 ? 4 : (NC <= 8 ? 3 : (NC <= 12 ? 2 : 1)))
+                                                             : (RS * NC <= 16 ? 2 : 1))) void k_kv8_step(Kv8AttnArgs a) {
     constexpr int KS = (NC + 3) / 4, HG = 4 * RS;
     extern __shared__ __align__(16) float lds[];                 // red [SW][HG][D], ml [SW][HG][2], the rows' bytes for RS > 1
     const int D = a.c.D, nc = D / 16, lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -432,7 +453,8 @@ __global__ __launch_bounds__(64 * SW, SW == 8 ? 2 : (RS == 1 ? (NC <= 4 ? 4 : (N
     const int nrow = rows - R0 < HG ? rows - R0 : HG;
     const int full = a.t.pos[i] < 0 ? 0 : a.t.pos[i], len = full < a.max_len ? full : a.max_len;
     const int64_t at0 = (int64_t) full - r.all;
-    const Kv8Seen first = kv8_seen(at0 + R0 / a.rep, len, a.window), last = kv8_seen(at0 + (R0 + nrow - 1) / a.rep, len, a.window);
+    const Kv8Seen first = kv8_seen(at0 + R0 / a.rep, len, a.window);
+    const Kv8Seen last = kv8_seen(at0 + (R0 + nrow - 1) / a.rep, len, a.window);
     const int64_t c0 = kv8_start(at0, len, a.window) + (int64_t) c * a.C, c1 = c0 + a.C;
     const int lo = first.lo > c0 ? first.lo : (int) (c0 < last.hi ? c0 : last.hi), hi = last.hi < c1 ? last.hi : (int) c1;
     if (a.nch > 1 && lo >= hi) return;
@@ -489,7 +511,7 @@ __global__ __launch_bounds__(64 * SW, SW == 8 ? 2 : (RS == 1 ? (NC <= 4 ? 4 : (N
     const uint32_t b = 3 - part, flip = part ? 0x80808080u : 0u;
     const uint32_t sel01 = 0x0c0c0000u | (4 + b) << 8 | b, sel23 = 0x00000c0cu | (4 + b) << 24 | b << 16;
     constexpr int bias = 0x00808080;          // makes the lower three bytes' signed digits unsigned
-    auto cut = [&](uint32_t y0, uint32_t y1, uint32_t y2, uint32_t y3) {           // byte `part` of four biased fixed-point numbers
+    auto cut = [&](uint32_t y0, uint32_t y1, uint32_t y2, uint32_t y3) {           // byte `part` of four biased numbers
         return (__builtin_amdgcn_perm(y1, y0, sel01) | __builtin_amdgcn_perm(y3, y2, sel23)) ^ flip;
     };
     auto cut_row = [&](int64_t base, i32x4 (&y)[KS]) {           // the bytes of a lane's row, and what a unit of them is worth
@@ -638,7 +660,8 @@ __global__ __launch_bounds__(64 * SW, SW == 8 ? 2 : (RS == 1 ? (NC <= 4 ? 4 : (N
             if (n * RS % 4 == 0) __builtin_amdgcn_sched_barrier(0);          // (four products' results at a time)
 #pragma unroll
             for (int k = 0; k < RS; k++) {
-                const i32x4 d = __builtin_amdgcn_mfma_i32_16x16x64_i8(pa[k], __builtin_bit_cast(i32x4, vr[n]), (i32x4){0, 0, 0, 0}, 0, 0, 0);
+                const i32x4 v = __builtin_bit_cast(i32x4, vr[n]);
+                const i32x4 d = __builtin_amdgcn_mfma_i32_16x16x64_i8(pa[k], v, (i32x4){0, 0, 0, 0}, 0, 0, 0);
                 acc[k][n] = fmaf((float) ((d[0] << 8) + d[1]), fh[k], acc[k][n]);
                 acc[k][n] = fmaf((float) ((d[2] << 8) + d[3]), fl[k], acc[k][n]);
             }
@@ -692,16 +715,24 @@ __global__ __launch_bounds__(64 * SW, SW == 8 ? 2 : (RS == 1 ? (NC <= 4 ? 4 : (N
     }
 }
 
-// Many query rows (prompts): bound by the matrix cores and, nearly as much, by the softmax's vector work.
-// A workgroup takes 128 rows (token, head of the kv head g), 32 a wave, and goes through the pages
-// that they see; a page's codes become fp16 (exact) in LDS once for its 4 waves, in the order that the
-// matrix instructions take them, two pages deep with the next one's codes in registers. A wave forms
-// S^T = K q^T: lane (row n, half) then holds tokens 32 T + 8 i + 4 half + c, which, V's tokens being taken in
-// the same order, is the operand of O^T = V^T P^T without a move across lanes. Rounding: q (bf16) is
+// Many query rows (prompts): bound by the matrix cores and the softmax's vector work together: the products of
+// a page and 32 rows take 1024 cycles of a SIMD (D = 128), the rest of it 1150, and two waves of a SIMD take the
+// sum of both, in whatever order they are run (alternating them by barriers: 397 us where this takes 352).
+// A workgroup takes 32 WR rows (token, head of the kv head g), 32 a wave, and goes through the pages
+// that they see; a page's codes become fp16 (exact) in LDS once for its waves, in the order that the
+// matrix instructions take them, two pages deep with the next one's codes in registers: they are converted and stored
+// between the products of the scores, whose time hides it (by themselves after them: 512 tokens of 40 / 8 heads over
+// 32768 371 us, so 352; 8 prompts at D = 256 242, 212). WV waves: 8 share a page's conversion, and with KS = 2 are two
+// groups of 4 with every second page each, joined at the end; which of them is taken where is attn_plan's rule.
+// A wave forms S^T = K q^T: lane (row n, half) then holds tokens 32 T + 8 i + 4 half + c, which, V's tokens being
+// taken in the same order, is the operand of O^T = V^T P^T without a move across lanes. Rounding: q (bf16) is
 // exact in fp16 after scaling its row by a power of two (to 2^-32 of the largest); the weights are
 // rounded to fp16 (half a step 2^-12 of each, and the row's sum adds the rounded ones), below the
-// output's bf16; sums, maxima and o are fp32. The V scale rides on the weights, relative to a power of
-// two 2^eref that follows it; a row's reference maximum moves only when a score passes it by 2^3.
+// output's bf16; F32: q and the weights in two fp16 parts each, to 2^-22, twice the products. Sums, maxima and o are
+// fp32. The V scale rides on the weights, relative to a power of two 2^eref that follows it; a row's reference maximum
+// moves only when a score passes it by 2^3.
+// 32 / 8 heads of 128 bf16: 2048 tokens on themselves 61 us (560 TFLOP/s), 8192 620 us (885), 512 of 40 / 8 over
+// 32768 352 us (950; a large bf16 product reaches 1372). 2048 in fp32: 114 us.
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -739,7 +770,8 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 && !F32 ? 8 / WV : 1) void k_kv8_t
     const int R0 = z * TR, nrow = rows - R0 < TR ? rows - R0 : TR;
     const int full = a.t.pos[i] < 0 ? 0 : a.t.pos[i], len = full < a.max_len ? full : a.max_len;
     const int64_t at0 = (int64_t) full - r.all;
-    const Kv8Seen first = kv8_seen(at0 + R0 / a.rep, len, a.window), last = kv8_seen(at0 + (R0 + nrow - 1) / a.rep, len, a.window);
+    const Kv8Seen first = kv8_seen(at0 + R0 / a.rep, len, a.window);
+    const Kv8Seen last = kv8_seen(at0 + (R0 + nrow - 1) / a.rep, len, a.window);
     const int64_t c0 = kv8_start(at0, len, a.window) + (int64_t) c * a.C, c1 = c0 + a.C;
     const int lo = first.lo > c0 ? first.lo : (int) (c0 < last.hi ? c0 : last.hi), hi = last.hi < c1 ? last.hi : (int) c1;
     if (a.nch > 1 && lo >= hi) return;
@@ -778,7 +810,8 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 && !F32 ? 8 / WV : 1) void k_kv8_t
     };
     auto store_piece = [&](int k, uint4 * to) {                  // a quarter of a unit: 4 codes of a lane
         const int u = k >> 2, e = k & 3;
-        codes_f16(e == 0 ? raw[u].x : (e == 1 ? raw[u].y : (e == 2 ? raw[u].z : raw[u].w)), e & 1 ? piece.z : piece.x, e & 1 ? piece.w : piece.y);
+        const uint32_t x = e == 0 ? raw[u].x : (e == 1 ? raw[u].y : (e == 2 ? raw[u].z : raw[u].w));
+        codes_f16(x, e & 1 ? piece.z : piece.x, e & 1 ? piece.w : piece.y);
         if (e & 1) to[dst[u][e >> 1]] = piece;
     };
     auto store = [&](uint4 * to) {
@@ -797,11 +830,13 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 && !F32 ? 8 / WV : 1) void k_kv8_t
         lls = bad ? nan : __builtin_amdgcn_logf(p[1] < 1e-36f ? 1e-36f : p[1]);
     };
     auto lane_at = [&](int n) {
-        return (int64_t) ((uint64_t) (uint32_t) __builtin_amdgcn_readlane((int) (lat >> 32), n) << 32 | (uint32_t) __builtin_amdgcn_readlane((int) lat, n));
+        const uint32_t hi = __builtin_amdgcn_readlane((int) (lat >> 32), n), lo = __builtin_amdgcn_readlane((int) lat, n);
+        return (int64_t) ((uint64_t) hi << 32 | lo);
     };
     auto lane_f = [&](float v, int n) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), n)); };
 
-    const int p0 = pbeg + grp, np = pend > p0 ? (pend - p0 + KS - 1) / KS : 0, rounds = pend > pbeg ? (pend - pbeg + KS - 1) / KS : 0;
+    const int p0 = pbeg + grp, np = pend > p0 ? (pend - p0 + KS - 1) / KS : 0;
+    const int rounds = pend > pbeg ? (pend - pbeg + KS - 1) / KS : 0;
     float qk[3] = {0.f, 0.f, 0.f}, qs[3] = {0.f, 0.f, 0.f};      // scales of pages n .. n + 2
     int64_t next = 0;                         // where page n + 2 is
     if (np > 0) {                             // (the first page's codes are on their way while q is prepared)
@@ -821,7 +856,8 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 && !F32 ? 8 / WV : 1) void k_kv8_t
     const Kv8Seen mine = kv8_seen(at0 + j, len, a.window);
     const bool live = w * 32 < nrow;                             // a wave behind the last row only loads
     const int wl = live ? w * 32 : nrow - 1, wh = w * 32 + 31 < nrow ? w * 32 + 31 : nrow - 1;
-    const Kv8Seen wfirst = kv8_seen(at0 + (R0 + wl) / a.rep, len, a.window), wlast = kv8_seen(at0 + (R0 + wh) / a.rep, len, a.window);
+    const Kv8Seen wfirst = kv8_seen(at0 + (R0 + wl) / a.rep, len, a.window);
+    const Kv8Seen wlast = kv8_seen(at0 + (R0 + wh) / a.rep, len, a.window);
     f16x8 q[PARTS][NC];
     float rowf;
     {
@@ -874,7 +910,8 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 && !F32 ? 8 / WV : 1) void k_kv8_t
     auto k_step = [&](int k, uint4 fr) {
 #pragma unroll
         for (int y = 0; y < PARTS; y++)
-            sc[k / NC] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, fr), q[y][k % NC], k % NC || y ? sc[k / NC] : zero, 0, 0, 0);
+            sc[k / NC] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, fr), q[y][k % NC],
+                                                                k % NC || y ? sc[k / NC] : zero, 0, 0, 0);
     };
     // ... and of o's, of V: 16 tokens (T, v), 32 d each
     auto v_frag = [&](int k) { return 2 * NC + k % ND * 4 + k / ND; };
@@ -1014,7 +1051,8 @@ __global__ __launch_bounds__(64 * WV, NC <= 8 && !F32 ? 8 / WV : 1) void k_kv8_t
                 f32x2 y;
 #pragma unroll
                 for (int v = 0; v < 2; v++)
-                    y[v] = __builtin_amdgcn_exp2f(MASK ? fmaf(sc[T][2 * e + v] - base, LOG2E, lr) : fmaf(sc[T][2 * e + v], k, off));
+                    y[v] = __builtin_amdgcn_exp2f(MASK ? fmaf(sc[T][2 * e + v] - base, LOG2E, lr)
+                                                       : fmaf(sc[T][2 * e + v], k, off));
                 p[0][T][e] = __builtin_convertvector(y, f16x2);
                 sum = __builtin_amdgcn_fdot2(p[0][T][e], one, sum, false);
                 if (F32) {
@@ -1131,7 +1169,7 @@ __global__ __launch_bounds__(KT) void k_kv8_combine(Kv8AttnArgs a) {
     const int full = a.t.pos[i] < 0 ? 0 : a.t.pos[i], len = full < a.max_len ? full : a.max_len;
     const Kv8Seen s = kv8_seen((int64_t) full - r.all + j, len, a.window);
     const int at = kv8_start((int64_t) full - r.all, len, a.window);
-    const int ca = (s.lo - at) / a.C, cb = live && s.hi > s.lo ? (s.hi - 1 - at) / a.C + 1 : ca;             // the chunks that this row sees
+    const int ca = (s.lo - at) / a.C, cb = live && s.hi > s.lo ? (s.hi - 1 - at) / a.C + 1 : ca;             // this row's chunks
     const int64_t o = (r.row + (live ? j : 0)) * a.Hq + h;
     const float * wo = a.ws + o * a.nch * D, * wml = a.ws + a.t.T * a.Hq * a.nch * D + o * a.nch * 2;
     // (maxima are in powers of 2 without a mask, in powers of e with one: its lowest value has to fit)
@@ -1166,8 +1204,8 @@ __global__ __launch_bounds__(KT) void k_kv8_combine(Kv8AttnArgs a) {
     else __builtin_amdgcn_wave_barrier();
     if (live && part == 0 && lane < DL && d < D) {
         for (int k = 1; k < G; k++) y += sred[w + k / (64 / DL)][(k % (64 / DL)) * DL + lane];
-        const float f = den == 0.f ? 0.f : 1.f / den;
-        const float4 v = make_float4(den == 0.f ? 0.f : y[0] * f, den == 0.f ? 0.f : y[1] * f, den == 0.f ? 0.f : y[2] * f, den == 0.f ? 0.f : y[3] * f);
+        const float f = 1.f / den;
+        const float4 v = den == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(y[0] * f, y[1] * f, y[2] * f, y[3] * f);
         if (a.f32) *(float4 *) ((float *) a.out + o * D + d) = v;
         else *(uint2 *) ((uint16_t *) a.out + o * D + d) = make_uint2(pack_bf16(v.x, v.y), pack_bf16(v.z, v.w));
     }
@@ -1184,7 +1222,7 @@ __global__ __launch_bounds__(KT) void k_kv8_join(Kv8AttnArgs a) {
     const int full = a.t.pos[i] < 0 ? 0 : a.t.pos[i], len = full < a.max_len ? full : a.max_len;
     const Kv8Seen s = kv8_seen((int64_t) full - r.all + j, len, a.window);
     const int at = kv8_start((int64_t) full - r.all, len, a.window);
-    const int ca = (s.lo - at) / a.C, n = s.hi > s.lo ? (s.hi - 1 - at) / a.C + 1 - ca : 0;        // the chunks that this row sees
+    const int ca = (s.lo - at) / a.C, n = s.hi > s.lo ? (s.hi - 1 - at) / a.C + 1 - ca : 0;        // this row's chunks
     const int64_t o = (r.row + j) * a.Hq + h;
     const float * wo = a.ws + (o * a.nch + ca) * D + d, * wml = a.ws + a.t.T * a.Hq * a.nch * D + (o * a.nch + ca) * 2;
     const float unit = a.mask ? LOG2E : 1.f, sink = a.sinks ? a.sinks[h] * (a.mask ? 1.f : LOG2E) : -__builtin_inff();
@@ -1224,8 +1262,10 @@ AttnPlan attn_plan(int f32, int Hq, int D, int Hkv, int nseq, int max_n, int max
     const int64_t rows = (int64_t) max_n * (Hq / Hkv);
     p.tile = rows > 16 && (!f32 || D <= 128);                    // (fp32 at D > 128 has no registers for two parts of q)
     p.RS = rows <= 4 ? 1 : (rows <= 8 || D > 64 ? 2 : 4);        // (four sets' registers fit beside the codes of D = 64)
-    // The prompt kernel's workgroups: 8 waves over 256 rows where every row sees nearly the same tokens, 8 waves in two
-    // groups over 128 rows where there are no more, else 4 waves over 128 rows, which balance a causal triangle better.
+    // The prompt kernel's workgroups: 8 waves over 256 rows where every row sees nearly the same tokens (512 over 32768: 352
+    // us, in two groups 396); 8 waves in two groups of every second page over 128 rows where there are no more, or no
+    // more of these than CUs (1024 on themselves 34.7 -> 29.5 us, 1024 behind 1024 54.9 -> 46.8; of 320 such workgroups
+    // 20.2 -> 25.2); else 4 waves over 128 rows, which balance a causal triangle better (2048: 61 us, 256 rows 83).
     // (8 waves need whole units of a page: D up to 64 and from 97 to 128.)
     const bool eight = !f32 && (D <= 64 || (D > 96 && D <= 128));
     p.wv = eight && (rows <= 128 || (int64_t) max_n * 4 <= max_len) ? 8 : 4;
@@ -1234,7 +1274,9 @@ AttnPlan attn_plan(int f32, int Hq, int D, int Hkv, int nseq, int max_n, int max
     p.ks = two ? 2 : 1;
     const int group = p.tile ? 32 * p.wv / p.ks : 4 * p.RS;
     p.ngrp = (int) ((rows + group - 1) / group);
-    const int64_t wgs = (int64_t) Hkv * p.ngrp * nseq, eff = window > 0 ? std::min<int64_t>(max_len, (int64_t) window + max_n + KV8_PAGE - 2) : max_len;
+    const int64_t wgs = (int64_t) Hkv * p.ngrp * nseq;
+    // the most tokens of a sequence that the call's rows see, from the page of the first (kv8_start)
+    const int64_t eff = window > 0 ? std::min<int64_t>(max_len, (int64_t) window + max_n + KV8_PAGE - 2) : max_len;
     int64_t C;
     if (p.tile) {
         // Split along the tokens where the workgroups leave CUs without, in chunks of 512 tokens or more (2048 for a twofold
@@ -1249,8 +1291,9 @@ AttnPlan attn_plan(int f32, int Hq, int D, int Hkv, int nseq, int max_n, int max
                 if (used(n) > 1.15 * used(nch)) nch = n;
         C = ((eff + nch - 1) / nch + KV8_PAGE - 1) / KV8_PAGE * KV8_PAGE;
     } else {
-        const int64_t single = 2048;
-        C = eff <= single ? eff : std::min<int64_t>(std::max<int64_t>(eff * wgs / 512, 512), 2048);
+        // whole up to 2048 tokens (2000 of one sequence: 11.0 us; 4000 in 8 chunks 7.4, the join 3.3 and its launch), then in
+        // chunks of 512 to 2048 tokens, so that the workgroups go around the 256 CUs twice
+        C = eff <= 2048 ? eff : std::min<int64_t>(std::max<int64_t>(eff * wgs / 512, 512), 2048);
         // eight waves a workgroup where the workgroups leave CUs without
         p.sw = wgs * ((eff + C - 1) / C) <= 256 && D <= 128 ? 8 : 4;
         // non-temporal loads where the codes are more than the caches would keep for another call (MB, us without -> with: 1070
@@ -1313,7 +1356,7 @@ hipError_t launch_kv8_write(const Kv8Cache & c, const Kv8Table & t, const void *
     WriteArgs a{c, t, {k, v}, {krs, vrs}, {khs, vhs}, (int) (((int64_t) t.max_n + KV8_PAGE - 2) / KV8_PAGE + 1)};
     if (!grid_fits((int64_t) a.W * c.Hkv, t.nseq)) return hipErrorInvalidValue;
     const dim3 grid((unsigned) (a.W * c.Hkv), (unsigned) t.nseq);
-    const size_t lds = KV8_PAGE * c.D;
+    const size_t lds = (KV8_PAGE + 4) * c.D;
     if (f32 && c.D <= 128) k_kv8_write<true, 1><<<grid, KT, lds, s>>>(a);
     else if (f32) k_kv8_write<true, 2><<<grid, KT, lds, s>>>(a);
     else if (c.D <= 128) k_kv8_write<false, 1><<<grid, KT, lds, s>>>(a);
@@ -1325,8 +1368,8 @@ hipError_t launch_kv8_read(const Kv8Cache & c, const Kv8Table & t, void * k, voi
     ReadArgs a{c, t, {k, v}, (int) (((int64_t) t.max_n + KV8_PAGE - 2) / KV8_PAGE + 1)};
     if (!grid_fits((int64_t) a.W * c.Hkv, t.nseq)) return hipErrorInvalidValue;
     const dim3 grid((unsigned) (a.W * c.Hkv), (unsigned) t.nseq);
-    if (f32) k_kv8_read<true><<<grid, KT, KV8_PAGE * c.D, s>>>(a);
-    else k_kv8_read<false><<<grid, KT, KV8_PAGE * c.D, s>>>(a);
+    if (f32) k_kv8_read<true><<<grid, KT, (KV8_PAGE + 4) * c.D, s>>>(a);
+    else k_kv8_read<false><<<grid, KT, (KV8_PAGE + 4) * c.D, s>>>(a);
     return hipGetLastError();
 }
 
@@ -1339,8 +1382,10 @@ hipError_t launch_kv8_attn(const Kv8Cache & c, const Kv8Table & t, const void * 
                            int max_len, const float * mask, int64_t mld, const float * sinks, int window, float scale,
                            void * out, void * ws, hipStream_t s) {
     const AttnPlan p = attn_plan(f32, Hq, c.D, c.Hkv, t.nseq, t.max_n, max_len, window);
-    Kv8AttnArgs a{c, t, q, out, mask, sinks, (float *) ws, qrs, qhs, mld, scale, Hq, Hq / c.Hkv, max_len, window, f32, p.C, p.nch, p.fold};
-    if (!grid_fits((int64_t) Hq * t.max_n * (c.D / 4) / KT + 1, t.nseq) || !grid_fits((int64_t) Hq * t.max_n, t.nseq) || !grid_fits((int64_t) c.Hkv * p.ngrp, t.nseq) || p.nch > 65535)
+    Kv8AttnArgs a{c, t, q, out, mask, sinks, (float *) ws, qrs, qhs, mld, scale, Hq, Hq / c.Hkv, max_len, window, f32, p.C,
+                  p.nch, p.fold};
+    // (rows times heads within a grid keeps the join's thread index, D / 4 times that, below 2^31)
+    if (!grid_fits((int64_t) Hq * t.max_n, t.nseq) || !grid_fits((int64_t) c.Hkv * p.ngrp, t.nseq) || p.nch > 65535)
         return hipErrorInvalidValue;
     const int nc = c.D / 16;
     hipError_t e = nc <= 4 ? run_attn<4>(a, p, s) : (nc <= 6 ? run_attn<6>(a, p, s) : (nc <= 8 ? run_attn<8>(a, p, s) :

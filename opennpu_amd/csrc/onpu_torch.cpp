@@ -1,7 +1,7 @@
 // opennpu_amd._kv8: the 8-bit key-value cache's calls for torch tensors (device.py kv8_write, kv8_read, kv8_attn),
 // checked here and handed to the C entries of include/onpu.h, whose addresses device.py binds. A decode
 // step's calls are bound by their issue: through ctypes and checks in Python kv8_attn took 9.9 us of the
-// host to issue, 3.3 of them the launch.
+// host to issue, here 4.2, 3.3 of them the launch.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
