@@ -109,10 +109,10 @@ __device__ __forceinline__ float scale_for(uint32_t bits) {
     return bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fmaxf(__uint_as_float(bits), KV8_TINY) / 127.f;
 }
 
-// Where word w of V's codes is in LDS: a lane turns the 8 words of 8 d, lanes differ in 16 d and in the token's quad,
-// which are 256 and 64 words apart; 4 words between every 64 leave 16 banks of 64 to them instead of 2
-// (8192 tokens x 8 x 128 bf16 written in 17.0 us, read in 10.9; without 17.8, 11.9).
-__device__ __forceinline__ int vt_at(int w) { return w + (w >> 6) * 4; }
+// Where word w of V's codes is in LDS: a lane turns the words of 4 or 8 d, lanes differ in 16 d and in the token's quad,
+// which are 256 and 64 words apart; 4 words between every 256 leave 16 banks of 64 to them instead of 2
+// (8192 tokens x 8 x 128 bf16 written in 17.0 us, read in 10.6; without 17.8, 11.9).
+__device__ __forceinline__ int vt_at(int w) { return w + (w >> 8) * 4; }
 
 // NQ: D up to 128 NQ
 template <bool F32, int NQ>
@@ -294,9 +294,9 @@ __global__ __launch_bounds__(KT) void k_kv8_write(WriteArgs a) {
 // ------------------------------------------------------------------ read
 // A workgroup per (page, kv head, sequence): value = code * scale, rounded once (bf16: that rounded
 // again); code + 128 by an unsigned byte's conversion, less 128 in the product's fma, whose one rounding is
-// the product's. A page that the table does not have reads as NaN. Bound by the bytes: a lane writes 16 d
-// of a K token and 8 d of 4 V tokens, V's words turned through LDS. 8192 tokens x 8 x 128 to bf16: 10.9 us for 50 MB,
-// 4.6 TB/s.
+// the product's. A page that the table does not have reads as NaN. Bound by the bytes: a lane writes 16 bytes of a
+// K row or of 4 V rows, so that a wave's stores are whole lines (16 d a lane, fp32: 16 prompts of up to 1500 of
+// 4 x 96 15.9 us, so 11.6), V's words turned through LDS. 8192 tokens x 8 x 128 to bf16: 10.6 us for 50 MB, 4.7 TB/s.
 struct ReadArgs {
     Kv8Cache c;
     Kv8Table t;
@@ -311,7 +311,7 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
 }
 
-// N values (8 or 16) to row `at` of y
+// N values (fp32 4, bf16 8: 16 bytes) to `at` of y
 template <bool F32, int N> __device__ __forceinline__ void put(void * y, int64_t at, const float (&v)[N]) {
     if (F32) {
 #pragma unroll
@@ -327,7 +327,7 @@ template <bool F32, int N> __device__ __forceinline__ void put(void * y, int64_t
 template <bool F32>
 __global__ __launch_bounds__(KT) void k_kv8_read(ReadArgs a) {
     extern __shared__ __align__(16) uint32_t vt[];               // V's 64 D codes (vt_at)
-    const int D = a.c.D, NC = D / 16, t = threadIdx.x, g = blockIdx.x % a.c.Hkv, w = blockIdx.x / a.c.Hkv, i = blockIdx.y;
+    const int D = a.c.D, t = threadIdx.x, g = blockIdx.x % a.c.Hkv, w = blockIdx.x / a.c.Hkv, i = blockIdx.y;
     const Kv8Rows r = kv8_rows(a.t.off, i, a.t.T, a.t.max_n);
     const int64_t p0 = a.t.pos[i], pg = (p0 - (p0 & (KV8_PAGE - 1))) / KV8_PAGE + w, base = pg * KV8_PAGE;
     if (base >= p0 + r.n) return;
@@ -338,28 +338,33 @@ __global__ __launch_bounds__(KT) void k_kv8_read(ReadArgs a) {
     const float * sc = a.c.scales + ((int64_t) (id < 0 ? 0 : id) * a.c.Hkv + g) * 2;
     for (int u = t; u < 4 * D; u += KT) *(uint4 *) (vt + vt_at(4 * u)) = ((const uint4 *) (in + KV8_PAGE * D))[u];
     const float nan = __uint_as_float(0x7fc00000u), sk = id < 0 ? nan : sc[0], sv = id < 0 ? nan : sc[1];
-    for (int u = s0 * NC + t; u < s1 * NC; u += KT) {
-        const int tok = u / NC, d = u % NC * 16;
-        const uint4 c = *(const uint4 *) (in + kv8_k_at(D, tok, d));
-        const uint32_t x[4] = {c.x ^ 0x80808080u, c.y ^ 0x80808080u, c.z ^ 0x80808080u, c.w ^ 0x80808080u};
-        float v[16];
+    constexpr int E = F32 ? 4 : 8;            // 16 bytes of a row a lane, so that a wave's stores are whole lines
+    const int per = D / E;
+    for (int u = s0 * per + t; u < s1 * per; u += KT) {
+        const int tok = u / per, d = u % per * E;
+        const uint32_t * p = (const uint32_t *) (in + kv8_k_at(D, tok, d));
+        float v[E];
 #pragma unroll
-        for (int e = 0; e < 16; e++) v[e] = fmaf((float) (x[e >> 2] >> (8 * (e & 3)) & 255), sk, -128.f * sk);
-        put<F32, 16>(a.y[0], ((row0 + tok) * a.c.Hkv + g) * D + d, v);
+        for (int k = 0; k < E / 4; k++) {
+            const uint32_t x = p[k] ^ 0x80808080u;
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[4 * k + e] = fmaf((float) (x >> (8 * e) & 255), sk, -128.f * sk);
+        }
+        put<F32, E>(a.y[0], ((row0 + tok) * a.c.Hkv + g) * D + d, v);
     }
     __syncthreads();
-    for (int u = (s0 >> 2) * 2 * NC + t; u < ((s1 + 3) >> 2) * 2 * NC; u += KT) {
-        const int q = u / (2 * NC), d = u % (2 * NC) * 8;
-        uint32_t x[8];
+    for (int u = (s0 >> 2) * per + t; u < ((s1 + 3) >> 2) * per; u += KT) {
+        const int q = u / per, d = u % per * E;
+        uint32_t x[E];
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = vt[vt_at(kv8_v_at(D, 4 * q, d + e) / 4)] ^ 0x80808080u;
+        for (int e = 0; e < E; e++) x[e] = vt[vt_at(kv8_v_at(D, 4 * q, d + e) / 4)] ^ 0x80808080u;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             if (4 * q + k < s0 || 4 * q + k >= s1) continue;
-            float v[8];
+            float v[E];
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = fmaf((float) (x[e] >> (8 * k) & 255), sv, -128.f * sv);
-            put<F32, 8>(a.y[1], ((row0 + 4 * q + k) * a.c.Hkv + g) * D + d, v);
+            for (int e = 0; e < E; e++) v[e] = fmaf((float) (x[e] >> (8 * k) & 255), sv, -128.f * sv);
+            put<F32, E>(a.y[1], ((row0 + 4 * q + k) * a.c.Hkv + g) * D + d, v);
         }
     }
 }
@@ -1356,7 +1361,7 @@ hipError_t launch_kv8_write(const Kv8Cache & c, const Kv8Table & t, const void *
     WriteArgs a{c, t, {k, v}, {krs, vrs}, {khs, vhs}, (int) (((int64_t) t.max_n + KV8_PAGE - 2) / KV8_PAGE + 1)};
     if (!grid_fits((int64_t) a.W * c.Hkv, t.nseq)) return hipErrorInvalidValue;
     const dim3 grid((unsigned) (a.W * c.Hkv), (unsigned) t.nseq);
-    const size_t lds = (KV8_PAGE + 4) * c.D;
+    const size_t lds = (KV8_PAGE + 1) * c.D;
     if (f32 && c.D <= 128) k_kv8_write<true, 1><<<grid, KT, lds, s>>>(a);
     else if (f32) k_kv8_write<true, 2><<<grid, KT, lds, s>>>(a);
     else if (c.D <= 128) k_kv8_write<false, 1><<<grid, KT, lds, s>>>(a);
@@ -1368,8 +1373,8 @@ hipError_t launch_kv8_read(const Kv8Cache & c, const Kv8Table & t, void * k, voi
     ReadArgs a{c, t, {k, v}, (int) (((int64_t) t.max_n + KV8_PAGE - 2) / KV8_PAGE + 1)};
     if (!grid_fits((int64_t) a.W * c.Hkv, t.nseq)) return hipErrorInvalidValue;
     const dim3 grid((unsigned) (a.W * c.Hkv), (unsigned) t.nseq);
-    if (f32) k_kv8_read<true><<<grid, KT, (KV8_PAGE + 4) * c.D, s>>>(a);
-    else k_kv8_read<false><<<grid, KT, (KV8_PAGE + 4) * c.D, s>>>(a);
+    if (f32) k_kv8_read<true><<<grid, KT, (KV8_PAGE + 1) * c.D, s>>>(a);
+    else k_kv8_read<false><<<grid, KT, (KV8_PAGE + 1) * c.D, s>>>(a);
     return hipGetLastError();
 }
 
