@@ -284,10 +284,11 @@ def kv8_read(codes, scales, table, pos, rows, off=None, max_n=None, dtype=None, 
 
 def kv8_attn(q, codes, scales, table, lens, off=None, max_n=None, max_len=None, mask=None, sinks=None, window=0, scale=None,
              out=None, ws=None):
-    """Causal grouped-query attention over the cache (onpu_kv8_attn_dev): q (fp32 or bf16 [T][Hq][D]) are the last
-    rows off[i]:off[i + 1] (off None: T / sequences each) of sequence i's lens[i] cached tokens. max_n, max_len: the most query rows
-    and tokens of one sequence (default: as many as there are, and as the table holds; closer bounds run
-    faster). mask fp32 [sequences][>= max_len] is added to the scores, sinks fp32 [Hq] is a logit per head without a
+    """Causal grouped-query attention over the cache (onpu_kv8_attn_dev): q (fp32 or bf16 [T][Hq][D]) holds sequence i's
+    queries in rows off[i]:off[i + 1] (off None: T / sequences each), the last of its lens[i] cached tokens. max_n, max_len:
+    the most query rows and tokens of one sequence (default: as many as there are, and as the table holds; closer
+    bounds run faster). mask fp32 [sequences][>= max_len] is added to the scores, sinks fp32 [Hq] is a logit per head without a
     value, window the last positions a query sees (0: all). ws: a workspace of onpu_kv8_attn_ws_bytes bytes, one
-    per call in flight (default: torch's allocator). Returns out [T][Hq][D] in q's type."""
+    per call in flight (default: torch's allocator). Returns out [T][Hq][D] in q's type; for serving, no gradient
+    passes through it."""
     return (_KV8 or _kv8()).attn(q, codes, scales, table, lens, off, max_n, max_len, mask, sinks, window, scale, out, ws)

@@ -536,6 +536,38 @@ def test_attn_replay_streams_and_repeats(gpu, B, n, S):
             assert torch.equal(outs[0], want) and torch.equal(outs[1], want), r
 
 
+@pytest.mark.parametrize("n", [1, 12, 60])
+def test_attn_replay_of_windows_and_masks(gpu, n):
+    """a graph of a window's chunks and one of a masked call, replayed with lengths that move the window and with
+    another mask in the buffers"""
+    import torch
+    from opennpu_amd.device import kv8_attn
+    rng = np.random.default_rng(n)
+    table, pages = _table(rng, [9000, 9000])
+    codes, scales = _rand_cache(rng, pages, 2, 64)
+    gc, gs, gt, lens = _dev(codes), _dev(scales), _i32(table), _i32([9000, 8000])
+    q, mask = torch.randn((2 * n, 8, 64), device="cuda").bfloat16(), torch.zeros((2, 9000), device="cuda")
+    calls = [lambda o: kv8_attn(q, gc, gs, gt, lens, max_len=9000, window=2500, out=o),         # noqa: E731
+             lambda o: kv8_attn(q, gc, gs, gt, lens, max_len=9000, mask=mask, out=o)]           # noqa: E731
+    graphs, outs = [], []
+    for call in calls:
+        call(None)
+        outs.append(torch.zeros_like(q))
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            call(outs[-1])
+        graphs.append(g)
+    for at in ([9000, 63 + n], [2500, 2564], [6401, 8999]):
+        lens.copy_(_i32(at))
+        mask.copy_(torch.where(torch.rand(mask.shape, device="cuda") < 0.5, -float("inf"), 0.0))
+        for g, o, call in zip(graphs, outs, calls):
+            o.zero_()
+            g.replay()
+            want = call(None)
+            torch.cuda.synchronize()
+            assert torch.equal(o, want), at
+
+
 def test_attn_strided_queries_and_untouched_rows(gpu):
     """q as a view into a projection's output; rows behind the last sequence, and a sequence's rows past
     max_n, as they were"""
@@ -659,3 +691,14 @@ def test_argument_errors(gpu):
             kv8_attn(q, c, s, t, p, **kw)
     with pytest.raises(RuntimeError, match="multiple of Hkv"):
         kv8_attn(q[:, :7], c, s, t, p)
+    for bad in ([None, c, s, t, p], [q, [1], s, t, p], [q, c, s, None, p], [q, c, s, t, 5], [q.cpu(), c, s, t, p]):
+        with pytest.raises(ValueError):
+            kv8_attn(*bad)
+    for kw in (dict(window=1.5), dict(max_len="9"), dict(scale="x")):
+        with pytest.raises(TypeError):
+            kv8_attn(q, c, s, t, p, **kw)
+    for kw in (dict(window=2 ** 40), dict(off=_i32([0, 2, 4]), max_n=2 ** 40), dict(ws=3), dict(out=1)):
+        with pytest.raises(ValueError):
+            kv8_attn(q, c, s, t, p, **kw)
+    with pytest.raises(RuntimeError, match="workspace"):
+        kv8_attn(q, c, s, _i32(np.zeros((2, 200))), p, ws=torch.empty((16,), dtype=torch.uint8, device="cuda"))
