@@ -1284,14 +1284,19 @@ AttnPlan attn_plan(int f32, int Hq, int D, int Hkv, int nseq, int max_n, int max
     const int64_t eff = window > 0 ? std::min<int64_t>(max_len, (int64_t) window + max_n + KV8_PAGE - 2) : max_len;
     int64_t C;
     if (p.tile) {
-        // Split along the tokens where the workgroups leave CUs without, in chunks of 512 tokens or more (2048 for a twofold
-        // split, whose gain the partials and the join cost again: 1024 tokens on themselves 34 us whole, 31 + 22 in two),
-        // and further where whole rounds of the workgroups come out fuller.
+        // Split along the tokens where the workgroups leave CUs without, in chunks of 512 tokens or more; where every row
+        // sees nearly the same tokens, of 256 up to 16 chunks and of 128 up to 8 (32 rows of 8 heads at D = 256 over 2000 in 4
+        // chunks 36.8 us, in 8 27.8; 17 tokens over 1000 whole 23.6, in 8 16.0; but 32 tokens over 8000 in 16 25.2, in 32
+        // 28.0: the partials). 2048 tokens or more for a twofold split, whose gain the partials and the join cost again.
+        // And further where whole rounds of the workgroups come out fuller.
         const int64_t slots = p.wv == 8 || D > 128 || f32 ? 256 : 512;
         auto used = [&](int64_t n) { return (double) (wgs * n) / (double) ((wgs * n + slots - 1) / slots * slots); };
-        int64_t nch = std::min<int64_t>(std::max<int64_t>(slots / wgs, 1), (eff + 511) / 512);
+        const bool flat = (int64_t) max_n * 4 <= eff;
+        int64_t most = (eff + 511) / 512;
+        if (flat) most = std::max(most, std::max(std::min<int64_t>((eff + 255) / 256, 16), std::min<int64_t>((eff + 127) / 128, 8)));
+        int64_t nch = std::min(std::max<int64_t>(slots / wgs, 1), most);
         if (nch == 2 && eff < 4096) nch = 1;
-        if ((int64_t) max_n * 4 <= max_len)
+        if (flat)
             for (int64_t n = nch + 1; n <= 8 && eff / n >= 2048; n++)
                 if (used(n) > 1.15 * used(nch)) nch = n;
         C = ((eff + nch - 1) / nch + KV8_PAGE - 1) / KV8_PAGE * KV8_PAGE;
